@@ -383,6 +383,114 @@ int tb200_mma_issue_probe(int64_t* out_clocks, int n, int a_in_tmem, int repetit
 #define TB200_DECODE_KERNEL_CP_ASYNC 2  /* gqa_decode_kernel: every thread loads with cp.async */
 int tb200_gqa_decode_last_kernel(void);
 
+/* ---------------------------------------------------------------------------
+ * Paged KV cache: block tables and slot maps of one step, built on the device.  (No counterpart in the
+ * reference, whose paged operators take finished tables, src/tileops/ops/attention/gqa.py:765-1157.)
+ *
+ * Request b holds seq_lens[b] tokens and appends new_lens[b].  It needs
+ * ceil((seq + new) / page_size) - ceil(seq / page_size) more pages, which come off the top of the stack
+ * free_pages[0 .. *free_count), in the order of the requests; a request is granted when its lengths make sense
+ * (neither is negative, the sum fits the width of the table) and it needs no page or the stack holds enough for it
+ * and the requests in front of it.
+ *   block_table       [batch, block_table_stride] int32; the entries of granted new pages are written, no others
+ *   cu_seqlens        [batch + 1]      exclusive sums of max(new_lens, 0): the packed batch's row ranges
+ *   slots, positions  [total_tokens]   row t (request b, its i-th new token): position seq_lens[b] + i and
+ *                     block_table[b][position / page_size] * page_size + position % page_size.  Slot -1 in the rows of a
+ *                     request that is not granted; slot -1, position 0 in rows behind the last request's
+ *   seq_lens_after    [batch]          seq + new where granted, else seq; may be seq_lens
+ *   free_count_after  [1]              may be free_count
+ *   granted           [batch]          1 or 0
+ *   free_pages, free_count, free_count_after all NULL: block_table holds every page already (a host that manages its
+ *   pages itself); nothing is allocated or written to it, and every request whose lengths make sense is granted
+ * batch <= 4096; max_pages_per_req * page_size <= 2^30; page ids * page_size must stay below 2^31.
+ *
+ * tb200_paged_kv_release puts the pages of the requests with finished[b] != 0 back on the stack (a request's last
+ * page first, never beyond free_capacity) and sets their seq_lens to 0; the table keeps its entries.
+ * ------------------------------------------------------------------------- */
+int tb200_paged_kv_plan(const int32_t* seq_lens, const int32_t* new_lens, int32_t* block_table,
+                        int64_t block_table_stride, const int32_t* free_pages, int64_t free_capacity,
+                        const int32_t* free_count, int32_t* cu_seqlens, int32_t* slots, int32_t* positions,
+                        int32_t* seq_lens_after, int32_t* free_count_after, int32_t* granted, int batch,
+                        int max_pages_per_req, int page_size, int total_tokens, void* stream);
+
+int tb200_paged_kv_release(const uint8_t* finished, int32_t* seq_lens, const int32_t* block_table,
+                           int64_t block_table_stride, int32_t* free_pages, int64_t free_capacity,
+                           int32_t* free_count, int batch, int max_pages_per_req, int page_size, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Per-head RMS norm and GPT-NeoX rotation of q and k in one pass, with the append to a paged cache.  (The rotation is
+ * that of RopeNeoxPositionIdsFwdOp, src/tileops/ops/rope.py:544-640; the reference has no operator that joins the norm.)
+ *   q [tokens, heads, dim], k, v [tokens, heads_kv, dim] dtype (F16 | BF16), strides in elements, last dim contiguous,
+ *   every row on a 16-byte boundary (parts of one fused projection's output serve as they are)
+ *   y = x * rsqrt(mean(x^2) + eps) * weight over a head's dim values; then the first rotary_dim values are rotated about
+ *   their midpoint by positions[t] * inv_freq[j]; fp32 throughout, angles in fp64, one rounding at the end
+ *   q_weight, k_weight [dim] of weight_dtype (dtype | F32), or NULL for ones
+ *   inv_turns [rotary_dim / 2] fp64: inv_freq / (2 pi)
+ *   q_out [tokens, heads, dim], k_out [tokens, heads_kv, dim] (or NULL) dtype, contiguous; neither may overlap an input
+ *   cache TB200_CACHE_16BIT: k and v rows also go to row slots[t] of k_cache / v_cache [pool_tokens, heads_kv, dim]
+ *   cache TB200_CACHE_INT4: they are quantised into k_cache = kv_pages (layout below); v_cache is not used
+ *   Slots outside [0, pool_tokens) are not written.  Slots of one call must be distinct: of two equal ones the
+ *   contents are undefined (each byte is one of the two rows').
+ * dim: a multiple of 8 up to 256 (64 or 128 for a 4-bit cache); rotary_dim: a multiple of 16 up to dim, or 0.
+ * ------------------------------------------------------------------------- */
+#define TB200_CACHE_NONE 0
+#define TB200_CACHE_16BIT 1
+#define TB200_CACHE_INT4 2
+int tb200_qk_norm_rope(const void* q, const void* k, const void* v, void* q_out, void* k_out, const void* q_weight,
+                       const void* k_weight, int weight_dtype, const double* inv_turns, const int32_t* positions,
+                       const int32_t* slots, void* k_cache, void* v_cache, int dtype, int cache, int tokens, int heads,
+                       int heads_kv, int dim, int rotary_dim, int64_t q_token_stride, int64_t q_head_stride,
+                       int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride,
+                       int page_size, int64_t pool_tokens, float eps, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Paged KV cache in 4 bits: one float16 (scale, offset) pair per token and KV head, for K and for V.  (No counterpart
+ * in the reference, whose quantised cache is e4m3 with scalar scales, src/tileops/kernels/attention/gqa_fwd.py:1005-1460.)
+ *   kv_pages uint8 [pool_pages, heads_kv, page_size * (dim + 8)], 16-byte aligned; per (page, KV head) page_size / 16
+ *   records of 16 tokens: K codes [16][dim / 2], V codes [16][dim / 2], params [16][4] float16 = K scale, K offset,
+ *   V scale, V offset.  Dim 2j is the low half of byte j, dim 2j + 1 the high half; value = scale * code + offset.
+ *   page_size: a multiple of 16.  dim: 64 or 128.
+ *
+ * append quantises rows into their slots (page * page_size + row of the page): lo, hi = smallest and largest value
+ * after clamping to +-65504; even slots offset = f16(lo), scale = f16((hi - lo) / 15), odd slots offset = f16(hi) and
+ * the scale negative; code = clamp(rint((x - offset) * (1 / scale)), 0, 15).  Rows with a NaN become NaN.  Slots outside
+ * [0, pool_tokens) are skipped; slots of one call must be distinct.
+ *
+ * gather reads it back: output rows cu_seqlens_kv[b] .. cu_seqlens_kv[b + 1] are request b's tokens 0, 1, ..: all of
+ * them from the cache (cache_seqlens NULL), or the first cache_seqlens[b] from the cache and the rest from rows
+ * cu_seqlens_new[b] .. of k_new / v_new.  scale * code + offset in fp32, rounded to dtype.  total_tokens bounds the rows
+ * (rows at or behind cu_seqlens_kv[batch] are left as they were); a page id outside the pool reads as NaN.
+ * ------------------------------------------------------------------------- */
+int tb200_int4_cache_append(const void* k, const void* v, const int32_t* slots, void* kv_pages, int dtype, int tokens,
+                            int heads_kv, int dim, int page_size, int64_t pool_tokens, int64_t k_token_stride,
+                            int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride, void* stream);
+
+int tb200_int4_cache_gather(const void* kv_pages, const int32_t* block_table, int64_t block_table_stride,
+                            int block_table_width, const int32_t* cu_seqlens_kv, const int32_t* cache_seqlens,
+                            const int32_t* cu_seqlens_new, const void* k_new, const void* v_new, void* k_out,
+                            void* v_out, int dtype, int total_tokens, int batch, int heads_kv, int dim, int page_size,
+                            int64_t pool_pages, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Single-token GQA decode over a paged 4-bit cache (layout above).
+ *   q [batch, heads, dim] q_dtype (F16 | BF16), o [batch, heads, dim] o_dtype (F16 | BF16 | F32), contiguous
+ *   lse [batch, heads] fp32 log2-domain or NULL; real_seqlen_kv [batch] int32 device
+ *   block_table [batch, block_table_stride] int32, of which the first block_table_width columns are a row's
+ * An empty sequence gives zeros (LSE -inf).  A page id outside [0, pool_pages), or a length beyond the table, makes that
+ * sequence's o and lse NaN; nothing outside the pool and the table is read.
+ * workspace: tb200_gqa_decode_int4_workspace_bytes() bytes, 256-byte aligned, the first
+ * TB200_DECODE_INT4_ZERO_BYTES(batch, heads, heads_kv) zeroed once; as for tb200_gqa_decode it belongs to one shape
+ * and one stream at a time.
+ * ------------------------------------------------------------------------- */
+#define TB200_DECODE_INT4_ZERO_BYTES(batch, heads, heads_kv) (((size_t)(batch) * (size_t)(heads) + 8) * 4)
+size_t tb200_gqa_decode_int4_workspace_bytes(int batch, int heads, int heads_kv, int dim);
+
+int tb200_gqa_decode_int4(const void* q, const void* kv_pages, void* o, float* lse, const int32_t* real_seqlen_kv,
+                          const int32_t* block_table, int64_t block_table_stride, int block_table_width, int q_dtype,
+                          int o_dtype, int batch, int heads, int heads_kv, int dim, int page_size, int64_t pool_pages,
+                          float sm_scale, float softcap, int flags, void* workspace, size_t workspace_bytes,
+                          void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -25,6 +25,8 @@ F16, BF16, E4M3, F32 = 0, 1, 2, 3
 # variant flags of tb200_gqa_decode (TB200_DECODE_* in include/tileops_b200.h)
 DECODE_WIDE_ON, DECODE_WIDE_OFF, DECODE_FP8_MMA, DECODE_NO_TMA = 1, 2, 4, 8
 DECODE_CHUNK_TILES_SHIFT = 8
+# kinds of cache of tb200_qk_norm_rope (TB200_CACHE_* in include/tileops_b200.h)
+CACHE_NONE, CACHE_16BIT, CACHE_INT4 = 0, 1, 2
 PREFILL_TWO_TILES = 1
 
 
@@ -119,6 +121,34 @@ SIGNATURES = {
         c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,      # k_pages v_pages k_new v_new k_out v_out
         c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p,  # cu_q cu_kv cache bt stride k_scale v_scale
         c_int, c_int, c_int, c_int, c_int, c_int, c_void_p]),          # dtype total_kv B Hkv D page stream
+    "tb200_paged_kv_plan": (c_int, [
+        c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p,   # seq_lens new_lens table stride free_pages capacity free_count
+        c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,     # cu slots positions seq_after free_after granted
+        c_int, c_int, c_int, c_int, c_void_p]),                        # batch max_pages page total stream
+    "tb200_paged_kv_release": (c_int, [
+        c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p,   # finished seq_lens table stride free_pages capacity free_count
+        c_int, c_int, c_int, c_void_p]),                               # batch max_pages page stream
+    "tb200_qk_norm_rope": (c_int, [
+        c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,               # q k v q_out k_out
+        c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p,        # q_weight k_weight weight_dtype inv_turns positions slots
+        c_void_p, c_void_p,                                            # k_cache v_cache
+        c_int, c_int, c_int, c_int, c_int, c_int, c_int,               # dtype cache tokens H Hkv D rotary_dim
+        c_int64, c_int64, c_int64, c_int64, c_int64, c_int64,          # q / k / v token and head strides
+        c_int, c_int64, c_float, c_void_p]),                           # page pool_tokens eps stream
+    "tb200_int4_cache_append": (c_int, [
+        c_void_p, c_void_p, c_void_p, c_void_p,                         # k v slots kv_pages
+        c_int, c_int, c_int, c_int, c_int, c_int64,                    # dtype tokens Hkv D page pool_tokens
+        c_int64, c_int64, c_int64, c_int64, c_void_p]),                # k / v token and head strides stream
+    "tb200_int4_cache_gather": (c_int, [
+        c_void_p, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_void_p,     # kv_pages table stride width cu_kv cached cu_new
+        c_void_p, c_void_p, c_void_p, c_void_p,                         # k_new v_new k_out v_out
+        c_int, c_int, c_int, c_int, c_int, c_int, c_int64, c_void_p]),  # dtype total B Hkv D page pool_pages stream
+    "tb200_gqa_decode_int4_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "tb200_gqa_decode_int4": (c_int, [
+        c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,               # q kv_pages o lse lens
+        c_void_p, c_int64, c_int, c_int, c_int,                        # table stride width q_dtype o_dtype
+        c_int, c_int, c_int, c_int, c_int, c_int64,                    # B H Hkv D page pool_pages
+        c_float, c_float, c_int, c_void_p, c_size_t, c_void_p]),       # sm_scale softcap flags ws bytes stream
     "tb200_mma_issue_probe": (c_int, [c_void_p, c_int, c_int, c_int, c_void_p]),
     "tb200_gqa_decode_last_kernel": (c_int, []),
     "tb200_fp8_cache_append": (c_int, [
@@ -168,6 +198,16 @@ def check(status: int, what: str) -> None:
 
 def ptr(t: "torch.Tensor | None") -> "int | None":
     return None if t is None else t.data_ptr()
+
+
+def launch(device: torch.device, fn, *args) -> int:
+    """``fn(*args, stream)`` on the current stream of ``device`` with that device current."""
+    index = device.index
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch._C._cuda_getDevice() == index:
+        return fn(*args, stream)
+    with torch.cuda.device(index):
+        return fn(*args, stream)
 
 
 def current_stream(device: torch.device) -> int:

@@ -1,0 +1,114 @@
+// Reads a 4-bit paged KV cache back as packed 16-bit K and V, sm_100a: the cache side of a chunked prefill, whose
+// tcgen05 attention kernel takes 16-bit operands.  value = scale * code + offset in fp32 (the product is exact), rounded
+// once.  HBM bound: dim + 8 bytes read and 4 dim written per token and KV head.
+#include "int4_cache.cuh"
+
+namespace tb200 {
+namespace {
+
+constexpr int kThreads = 128;
+
+struct GatherParams {
+  const unsigned char* pages;
+  const int32_t* table;
+  int64_t table_stride;
+  const int32_t* cu;        // [batch + 1]: request b owns output rows cu[b] .. cu[b + 1]
+  const int32_t* cached;    // NULL: all of a request's rows are cached; else its first cached[b] rows
+  const int32_t* cu_new;    // rows behind the cached ones come from k_new / v_new, request b from row cu_new[b] on
+  const void *k_new, *v_new;
+  void *k_out, *v_out;
+  int batch, heads_kv, page_size, table_width, pool_pages, total;
+};
+
+// One block per output token.  kLanes lanes hold a row, 8 values each.
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) int4_gather_kernel(GatherParams p) {
+  constexpr int kLanes = D / 8;
+  const int g = blockIdx.x;
+  if (g < p.cu[0] || g >= p.cu[p.batch]) return;   // `total` may be an upper bound: the host never reads the lengths
+  int lo = 0, hi = p.batch - 1;     // largest b with cu[b] <= g
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (p.cu[mid] <= g) lo = mid; else hi = mid - 1;
+  }
+  const int t = g - p.cu[lo];
+  const int lane = threadIdx.x % kLanes;
+  if (p.cached && t >= p.cached[lo]) {
+    const size_t src = size_t(p.cu_new[lo] + t - p.cached[lo]) * p.heads_kv * D;
+    for (int i = threadIdx.x * 8; i < p.heads_kv * D; i += kThreads * 8) {
+      *reinterpret_cast<uint4*>(static_cast<T*>(p.k_out) + size_t(g) * p.heads_kv * D + i) =
+          *reinterpret_cast<const uint4*>(static_cast<const T*>(p.k_new) + src + i);
+      *reinterpret_cast<uint4*>(static_cast<T*>(p.v_out) + size_t(g) * p.heads_kv * D + i) =
+          *reinterpret_cast<const uint4*>(static_cast<const T*>(p.v_new) + src + i);
+    }
+    return;
+  }
+  const int column = t / p.page_size;
+  const int page = column < p.table_width ? p.table[int64_t(lo) * p.table_stride + column] : -1;
+  const bool known = page >= 0 && page < p.pool_pages;   // a page outside the pool reads as NaN
+  const int off = t % p.page_size, tok = off % kInt4Tokens;
+  for (int r = threadIdx.x / kLanes; r < 2 * p.heads_kv; r += kThreads / kLanes) {
+    const int part = r >= p.heads_kv ? 1 : 0;
+    const int h = r - part * p.heads_kv;
+    uint32_t codes = 0, params = 0x7e007e00u;
+    if (known) {
+      const unsigned char* rec =
+          p.pages + ((size_t(page) * p.heads_kv + h) * size_t(p.page_size / kInt4Tokens) + off / kInt4Tokens) *
+                        size_t(int4_record_bytes(D));
+      codes = *reinterpret_cast<const uint32_t*>(rec + (part * kInt4Tokens + tok) * (D / 2) + lane * 4);
+      params = *reinterpret_cast<const uint32_t*>(rec + kInt4Tokens * D + tok * 8 + part * 4);
+    }
+    const float s = __half2float(__ushort_as_half(uint16_t(params)));
+    const float m = __half2float(__ushort_as_half(uint16_t(params >> 16)));
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = fmaf(s, float((codes >> (4 * e)) & 15u), m);
+    T* out = static_cast<T*>(part ? p.v_out : p.k_out) + (size_t(g) * p.heads_kv + h) * D + lane * 8;
+    *reinterpret_cast<uint4*>(out) =
+        make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
+  }
+}
+
+}  // namespace
+}  // namespace tb200
+
+using namespace tb200;
+
+extern "C" int tb200_int4_cache_gather(const void* kv_pages, const int32_t* block_table, int64_t block_table_stride,
+                                       int block_table_width, const int32_t* cu_seqlens_kv, const int32_t* cache_seqlens,
+                                       const int32_t* cu_seqlens_new, const void* k_new, const void* v_new, void* k_out,
+                                       void* v_out, int dtype, int total_tokens, int batch, int heads_kv, int dim,
+                                       int page_size, int64_t pool_pages, void* stream) {
+  if (total_tokens < 0 || batch <= 0 || heads_kv <= 0 || block_table_width <= 0)
+    TB200_FAIL(TB200_ERR_BAD_ARGUMENT, "batch, heads_kv and the table's width must be positive and total_tokens not negative");
+  if (dtype != TB200_BF16 && dtype != TB200_F16) TB200_FAIL(TB200_ERR_UNSUPPORTED, "dtype must be F16 or BF16");
+  if (dim != 64 && dim != 128) TB200_FAIL(TB200_ERR_UNSUPPORTED, "a 4-bit cache serves head dim 64 and 128, got %d", dim);
+  if (page_size <= 0 || page_size % kInt4Tokens != 0)
+    TB200_FAIL(TB200_ERR_UNSUPPORTED, "page_size must be a multiple of 16, got %d", page_size);
+  if (pool_pages < 0 || pool_pages > 0x7fffffffLL) TB200_FAIL(TB200_ERR_UNSUPPORTED, "too many pages");
+  if (total_tokens == 0) return TB200_OK;
+  if (!kv_pages || !block_table || !cu_seqlens_kv || !k_out || !v_out)
+    TB200_FAIL(TB200_ERR_BAD_ARGUMENT, "kv_pages, block_table, cu_seqlens_kv, k_out and v_out must be non-null");
+  if (cache_seqlens && (!cu_seqlens_new || !k_new || !v_new))
+    TB200_FAIL(TB200_ERR_BAD_ARGUMENT, "cache_seqlens comes with cu_seqlens_new, k_new and v_new");
+  if ((reinterpret_cast<uintptr_t>(kv_pages) | reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out) |
+       reinterpret_cast<uintptr_t>(k_new) | reinterpret_cast<uintptr_t>(v_new)) & 15)
+    TB200_FAIL(TB200_ERR_UNSUPPORTED, "tensors must start on 16-byte boundaries");
+  GatherParams p{};
+  p.pages = static_cast<const unsigned char*>(kv_pages);
+  p.table = block_table; p.table_stride = block_table_stride; p.table_width = block_table_width;
+  p.cu = cu_seqlens_kv; p.cached = cache_seqlens; p.cu_new = cu_seqlens_new; p.k_new = k_new; p.v_new = v_new;
+  p.k_out = k_out; p.v_out = v_out; p.batch = batch; p.heads_kv = heads_kv; p.page_size = page_size;
+  p.pool_pages = int(pool_pages); p.total = total_tokens;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool bf16 = dtype == TB200_BF16;
+  if (dim == 64) {
+    if (bf16) int4_gather_kernel<__nv_bfloat16, 64><<<total_tokens, kThreads, 0, s>>>(p);
+    else int4_gather_kernel<__half, 64><<<total_tokens, kThreads, 0, s>>>(p);
+  } else {
+    if (bf16) int4_gather_kernel<__nv_bfloat16, 128><<<total_tokens, kThreads, 0, s>>>(p);
+    else int4_gather_kernel<__half, 128><<<total_tokens, kThreads, 0, s>>>(p);
+  }
+  TB200_CUDA_CHECK(cudaGetLastError());
+  return TB200_OK;
+}

@@ -1,0 +1,77 @@
+// Layout and arithmetic of the 4-bit paged KV cache, shared by its writer (qk_norm_rope.cu), its reader for a
+// prefill (int4_cache.cu) and the decode attention (gqa_decode_int4.cu).
+//
+// kv_pages is uint8 [pages, heads_kv, page_size * (dim + 8)].  The bytes of one (page, KV head) are page_size / 16
+// RECORDS of 16 tokens:
+//     K codes  [16][dim / 2]     dim 2j of a token in the low half of byte j, dim 2j + 1 in the high half
+//     V codes  [16][dim / 2]
+//     params   [16][4] float16   K scale, K offset, V scale, V offset
+// and value = scale * code + offset.  A record is contiguous, so whatever the page size is a tile of the attention is
+// a few untiled bulk copies of whole records (2176 bytes at head dim 128, 1152 at 64), K, V and parameters together.
+//
+// Quantiser of one row (one token of one KV head), 15 steps between its smallest and largest value:
+//     lo, hi = min, max of the values clamped to +-65504
+//     even slots: offset = f16(lo), scale =  f16((hi - lo) / 15)
+//     odd slots:  offset = f16(hi), scale = -f16((hi - lo) / 15)
+//     code = clamp(rint((x - offset) * (1 / scale)), 0, 15), 0 where scale == 0
+// in fp32 with one reciprocal per row.  Both signs decode the same way.  They alternate because the attention sums
+// p * scale * code over thousands of tokens in tensor-core accumulators: codes are 0..15, so sums of one sign would
+// grow with the context while their useful part, the deviations from the mean, grows with its square root, and the
+// accumulator's rounding would eat into it; with alternating signs the means cancel.
+// A row that holds a NaN gets NaN parameters: its values, and the outputs that attend to it, are NaN.
+#pragma once
+
+#include "tb200_common.cuh"
+
+namespace tb200 {
+
+constexpr int kInt4Tokens = 16;   // tokens of a record
+__host__ __device__ constexpr int int4_record_bytes(int dim) { return kInt4Tokens * (dim + 8); }
+constexpr float kInt4Clamp = 65504.f;   // largest float16
+
+// First byte of the record that holds `slot`, for one KV head.  (slot >= 0)
+__device__ __forceinline__ size_t int4_record_of(int slot, int head, int heads_kv, int page_size, int dim) {
+  const int page = slot / page_size, off = slot - page * page_size;
+  return ((size_t(page) * heads_kv + head) * size_t(page_size / kInt4Tokens) + off / kInt4Tokens) *
+         size_t(int4_record_bytes(dim));
+}
+
+// Quantises 8 consecutive values of a row that kLanes neighbouring lanes hold together (8 values per lane, all lanes of
+// the group active).  Returns the 8 codes as 4 bytes; `params` (scale in the low half, offset in the high half) is the
+// same on every lane of the group.
+template <int kLanes>
+__device__ __forceinline__ uint32_t int4_quantise(const float (&v)[8], bool odd_slot, uint32_t& params) {
+  float x[8];
+  float lo = kInt4Clamp, hi = -kInt4Clamp;
+  bool bad = false;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    bad |= v[e] != v[e];
+    x[e] = fminf(fmaxf(v[e], -kInt4Clamp), kInt4Clamp);
+    lo = fminf(lo, x[e]);
+    hi = fmaxf(hi, x[e]);
+  }
+#pragma unroll
+  for (int o = 1; o < kLanes; o <<= 1) {
+    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+  }
+  const unsigned votes = __ballot_sync(0xffffffffu, bad);
+  const unsigned group = (kLanes == 32 ? 0xffffffffu : ((1u << kLanes) - 1u) << (threadIdx.x & 31 & ~(kLanes - 1)));
+  const __half step = __float2half_rn(__fdiv_rn(hi - lo, 15.f));
+  const __half scale = odd_slot ? __hneg(step) : step;
+  const __half offset = __float2half_rn(odd_slot ? hi : lo);
+  const float s = __half2float(scale), m = __half2float(offset);
+  const float inverse = s == 0.f ? 0.f : __frcp_rn(s);
+  uint32_t codes = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float c = fminf(fmaxf(rintf(__fmul_rn(x[e] - m, inverse)), 0.f), 15.f);
+    codes |= uint32_t(c) << (4 * e);
+  }
+  params = uint32_t(__half_as_ushort(scale)) | (uint32_t(__half_as_ushort(offset)) << 16);
+  if (votes & group) { params = 0x7e007e00u; codes = 0; }
+  return codes;
+}
+
+}  // namespace tb200

@@ -7,7 +7,7 @@ synchronise with the device.
 
 from __future__ import annotations
 
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
@@ -492,3 +492,371 @@ def mma_issue_probe(n: int = 128, a_in_tmem: bool = False, repetitions: int = 20
     if done < 0:
         raise N.NativeLibraryError("tb200_mma_issue_probe: the bounded wait for the last MMA ran out")
     return issued / (8.0 * repetitions), done / (8.0 * repetitions)
+
+
+# ---- paged KV cache: plans, per-head norm + rotation + append, the cache in 4 bits -------------------------------------
+
+class PagedKVPlan(NamedTuple):
+    """What :func:`paged_kv_plan` returns; every field is an int32 tensor on the GPU."""
+    cu_seqlens_q: torch.Tensor      # [B + 1]
+    slot_mapping: torch.Tensor      # [total_tokens], -1: not to be stored
+    positions: torch.Tensor         # [total_tokens]
+    seq_lens: torch.Tensor          # [B], after the step
+    free_count: Optional[torch.Tensor]   # [1], after the step
+    granted: torch.Tensor           # [B], 1 or 0
+
+
+def _check_vector(name: str, t: torch.Tensor, n: int, device: torch.device, dtype: torch.dtype = torch.int32) -> None:
+    if t.dtype != dtype or t.dim() != 1 or t.shape[0] != n:
+        raise ValueError(f"{name} must be {str(dtype)[6:]} with shape ({n},), got {t.dtype} {tuple(t.shape)}")
+    if t.device != device:
+        raise ValueError(f"{name} must be on {device}, got {t.device}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+
+
+def _check_table(block_table: torch.Tensor, batch: int, device: torch.device) -> None:
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != batch:
+        raise ValueError(f"block_table must be int32 with shape [{batch}, num_pages], got {block_table.dtype} "
+                         f"{tuple(block_table.shape)}")
+    if block_table.device != device:
+        raise ValueError(f"block_table must be on {device}, got {block_table.device}")
+    if block_table.shape[1] == 0:
+        raise ValueError("block_table must have at least one column")
+    if block_table.stride(1) != 1 and block_table.shape[1] > 1:
+        raise ValueError("the rows of block_table must be contiguous")
+
+
+def paged_kv_plan(seq_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor,
+                  free_pages: Optional[torch.Tensor], free_count: Optional[torch.Tensor], total_tokens: int, *,
+                  page_size: int, inplace: bool = False) -> PagedKVPlan:
+    """Plan of a step that appends ``new_lens[b]`` tokens to request b, built on the GPU without a host
+    synchronisation: pages come off the stack ``free_pages[0 .. free_count)`` into ``block_table`` (in place), and the
+    packed batch gets its row ranges, positions and cache slots (:class:`PagedKVPlan`).
+
+    ``total_tokens`` is the number of rows of the packed batch as the host knows it (at least ``sum(new_lens)``).  A
+    request whose lengths do not fit the table, or for which the stack is short, is not granted: its rows get slot -1 and
+    it keeps its length.  ``inplace=True`` updates ``seq_lens`` and ``free_count`` themselves (a step that a CUDA graph
+    replays).  With ``free_pages`` and ``free_count`` ``None`` the table is taken to hold every page already."""
+    _require_cuda(seq_lens=seq_lens)
+    device, batch, total = seq_lens.device, seq_lens.shape[0], int(total_tokens)
+    _check_vector("seq_lens", seq_lens, batch, device)
+    _check_vector("new_lens", new_lens, batch, device)
+    _check_table(block_table, batch, device)
+    if (free_pages is None) != (free_count is None):
+        raise ValueError("free_pages and free_count come together")
+    if free_pages is not None:
+        _check_vector("free_pages", free_pages, free_pages.numel(), device)
+        _check_vector("free_count", free_count, 1, device)
+    if total < 0:
+        raise ValueError("total_tokens must not be negative")
+    pad = -total % 4                                    # the maps start on 16-byte boundaries
+    buf = torch.empty(2 * (total + pad) + 3 * batch + 2, dtype=torch.int32, device=device)
+    slots, _, positions, _, cu, after, granted, count = buf.split_with_sizes(
+        [total, pad, total, pad, batch + 1, batch, batch, 1])
+    if inplace:
+        after, count = seq_lens, free_count
+    if free_count is None:
+        count = None
+    st = N.launch(device, N.lib().tb200_paged_kv_plan, seq_lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(),
+                  block_table.stride(0), N.ptr(free_pages), 0 if free_pages is None else free_pages.shape[0],
+                  N.ptr(free_count), cu.data_ptr(), slots.data_ptr(), positions.data_ptr(), after.data_ptr(),
+                  N.ptr(count), granted.data_ptr(), batch, block_table.shape[1], int(page_size), total)
+    N.check(st, "tb200_paged_kv_plan")
+    return PagedKVPlan(cu, slots, positions, after, count, granted)
+
+
+def paged_kv_release(finished: torch.Tensor, seq_lens: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor,
+                     free_count: torch.Tensor, *, page_size: int) -> None:
+    """Gives the pages of the requests with ``finished[b]`` (bool ``[B]``) back to the stack and sets their ``seq_lens`` to
+    0; ``free_pages``, ``free_count`` and ``seq_lens`` are updated in place on the GPU."""
+    _require_cuda(seq_lens=seq_lens)
+    device, batch = seq_lens.device, seq_lens.shape[0]
+    _check_vector("seq_lens", seq_lens, batch, device)
+    _check_vector("finished", finished, batch, device, torch.bool)
+    _check_table(block_table, batch, device)
+    _check_vector("free_pages", free_pages, free_pages.numel(), device)
+    _check_vector("free_count", free_count, 1, device)
+    st = N.launch(device, N.lib().tb200_paged_kv_release, finished.data_ptr(), seq_lens.data_ptr(),
+                  block_table.data_ptr(), block_table.stride(0), free_pages.data_ptr(), free_pages.shape[0],
+                  free_count.data_ptr(), batch, block_table.shape[1], int(page_size))
+    N.check(st, "tb200_paged_kv_release")
+
+
+def _rows(t: torch.Tensor) -> "Tuple[torch.Tensor, int, int]":
+    """``t [tokens, heads, dim]`` with its token and head strides, as it is when its rows start on 16-byte boundaries
+    (parts of a fused projection's output do), else a contiguous copy."""
+    tokens, heads, dim = t.shape
+    tok = t.stride(0) if tokens > 1 else heads * dim
+    head = t.stride(1) if heads > 1 else dim
+    if (t.stride(2) == 1 or dim == 1) and tok % 8 == 0 and head % 8 == 0 and t.data_ptr() % 16 == 0:
+        return t, tok, head
+    return t.clone(memory_format=torch.contiguous_format), heads * dim, dim
+
+
+def int4_page_bytes(page_size: int, dim: int) -> int:
+    """Bytes of one KV head's share of a page of the 4-bit cache: ``kv_pages`` is uint8
+    ``[pages, heads_kv, int4_page_bytes(page_size, dim)]``."""
+    return page_size * (dim + 8)
+
+
+def int4_cache_views(kv_pages: torch.Tensor, page_size: int, dim: int) -> "Tuple[torch.Tensor, ...]":
+    """Views of a 4-bit pool: K codes and V codes ``[pages, heads_kv, page_size / 16, 16, dim / 2]`` (uint8; dim 2j in
+    the low half of byte j) and the parameters ``[pages, heads_kv, page_size / 16, 16, 4]`` (float16: K scale, K offset,
+    V scale, V offset)."""
+    records = kv_pages.view(kv_pages.shape[0], kv_pages.shape[1], page_size // 16, 16 * (dim + 8))
+    k, v, params = records.split_with_sizes([8 * dim, 8 * dim, 128], -1)
+    return k.unflatten(-1, (16, dim // 2)), v.unflatten(-1, (16, dim // 2)), params.view(torch.float16).unflatten(-1, (16, 4))
+
+
+def _check_int4_pool(kv_pages: torch.Tensor, heads_kv: int, dim: int, page_size: int, device: torch.device) -> None:
+    if page_size <= 0 or page_size % 16 != 0:
+        raise ValueError(f"page_size must be a positive multiple of 16, got {page_size}")
+    if dim not in (64, 128):
+        raise ValueError(f"a 4-bit KV cache serves head dim 64 and 128, got {dim}")
+    want = (heads_kv, int4_page_bytes(page_size, dim))
+    if kv_pages.dtype != torch.uint8 or kv_pages.dim() != 3 or tuple(kv_pages.shape[1:]) != want:
+        raise ValueError(f"kv_pages must be uint8 with shape [pages, {want[0]}, {want[1]}], got {kv_pages.dtype} "
+                         f"{tuple(kv_pages.shape)}")
+    if kv_pages.device != device:
+        raise ValueError(f"kv_pages must be on {device}, got {kv_pages.device}")
+    if not kv_pages.is_contiguous() or kv_pages.data_ptr() % 16:
+        raise ValueError("kv_pages must be contiguous and start on a 16-byte boundary")
+
+
+def _check_kv_rows(k: torch.Tensor, v: torch.Tensor) -> None:
+    if k.dim() != 3 or v.shape != k.shape:
+        raise ValueError(f"k and v must have the same shape [tokens, heads_kv, dim], got {tuple(k.shape)} and "
+                         f"{tuple(v.shape)}")
+    if v.dtype != k.dtype:
+        raise ValueError(f"v must have the dtype of k, got {v.dtype} and {k.dtype}")
+    if v.device != k.device:
+        raise ValueError(f"v must be on {k.device}, got {v.device}")
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_turns: Optional[torch.Tensor], *,
+                 q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                 v: Optional[torch.Tensor] = None, slot_mapping: Optional[torch.Tensor] = None,
+                 k_pages: Optional[torch.Tensor] = None, v_pages: Optional[torch.Tensor] = None,
+                 kv_pages: Optional[torch.Tensor] = None, page_size: int = 0, return_k: bool = True):
+    """Per-head RMS norm of q ``[T,H,D]`` and k ``[T,Hkv,D]``, then the GPT-NeoX rotation of their first ``2 *
+    len(inv_turns)`` dims by ``positions[t]`` (int32 ``[T]``), in one pass; ``inv_turns`` is float64, frequencies over
+    2 pi (``None``: no rotation).  Computed in fp32, rounded once.  Returns q (and k when ``return_k``) as new contiguous
+    tensors.
+
+    With ``k_pages`` / ``v_pages`` (``[pool_tokens,Hkv,D]``, the dtype of q) or ``kv_pages`` (the 4-bit pool) the same
+    launch also stores k and v ``[T,Hkv,D]`` at the rows ``slot_mapping`` (int32 ``[T]``; rows outside the pool are
+    skipped, rows of one call must be distinct)."""
+    _require_cuda(q=q)
+    if q.dim() != 3 or k.dim() != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
+        raise ValueError(f"q must be [tokens, heads, dim] and k [tokens, heads_kv, dim], got {tuple(q.shape)} and "
+                         f"{tuple(k.shape)}")
+    device, dtype = q.device, q.dtype
+    if dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"Expected dtype torch.float16 or torch.bfloat16, got {dtype}")
+    if k.dtype != dtype or k.device != device:
+        raise ValueError(f"k must have the dtype and device of q, got {k.dtype} on {k.device}")
+    T, H, D = q.shape
+    Hkv = k.shape[1]
+    _check_vector("positions", positions, T, device)
+    half = 0
+    if inv_turns is not None:
+        half = inv_turns.numel()
+        _check_vector("inv_turns", inv_turns, half, device, torch.float64)
+    weight_dtype = dtype
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is not None:
+            if w.dtype != dtype and w.dtype != torch.float32:
+                raise ValueError(f"{name} must have the dtype of q or be torch.float32, got {w.dtype}")
+            _check_vector(name, w, D, device, w.dtype)
+            weight_dtype = w.dtype
+    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
+        raise ValueError("q_weight and k_weight must have the same dtype")
+    kind, pool_tokens, k_cache, v_cache, vs = N.CACHE_NONE, 0, None, None, (None, 0, 0)
+    if kv_pages is not None or k_pages is not None:
+        if v is None or slot_mapping is None:
+            raise ValueError("v and slot_mapping come with a cache")
+        _check_kv_rows(k, v)
+        _check_vector("slot_mapping", slot_mapping, T, device)
+        if kv_pages is not None:
+            if k_pages is not None or v_pages is not None:
+                raise ValueError("kv_pages cannot be combined with k_pages / v_pages")
+            _check_int4_pool(kv_pages, Hkv, D, page_size, device)
+            kind, k_cache, pool_tokens = N.CACHE_INT4, kv_pages.data_ptr(), kv_pages.shape[0] * page_size
+        else:
+            if v_pages is None:
+                raise ValueError("k_pages and v_pages come together")
+            for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
+                if t.dim() != 3 or tuple(t.shape[1:]) != (Hkv, D) or t.shape[0] != k_pages.shape[0] or t.dtype != dtype:
+                    raise ValueError(f"{name} must be [pool_tokens, {Hkv}, {D}] with dtype {dtype}, got {tuple(t.shape)} "
+                                     f"{t.dtype}")
+                if t.device != device or not t.is_contiguous() or t.data_ptr() % 16:
+                    raise ValueError(f"{name} must be contiguous, on {device}, and start on a 16-byte boundary")
+            kind, pool_tokens = N.CACHE_16BIT, k_pages.shape[0]
+            k_cache, v_cache = k_pages.data_ptr(), v_pages.data_ptr()
+        vs = _rows(v)
+    q_out = torch.empty((T, H, D), dtype=dtype, device=device)
+    k_out = torch.empty((T, Hkv, D), dtype=dtype, device=device) if return_k else None
+    (q, q_tok, q_head), (k, k_tok, k_head) = _rows(q), _rows(k)
+    st = N.launch(device, N.lib().tb200_qk_norm_rope, q.data_ptr(), k.data_ptr(), N.ptr(vs[0]), q_out.data_ptr(),
+                  N.ptr(k_out), N.ptr(q_weight), N.ptr(k_weight), N.dtype_code(weight_dtype), N.ptr(inv_turns),
+                  positions.data_ptr(), N.ptr(slot_mapping), k_cache, v_cache, N.dtype_code(dtype), kind, T, H, Hkv, D,
+                  2 * half, q_tok, q_head, k_tok, k_head, vs[1], vs[2], page_size, pool_tokens, eps)
+    N.check(st, "tb200_qk_norm_rope")
+    return (q_out, k_out) if return_k else q_out
+
+
+def int4_cache_append(k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tensor, kv_pages: torch.Tensor, *,
+                      page_size: int) -> None:
+    """Quantises k and v ``[T,Hkv,D]`` into the rows ``slot_mapping`` (int32 ``[T]``) of the 4-bit pool, in place: 15
+    steps between a row's smallest and largest value, one float16 scale and offset per token and KV head (error at most
+    half a step plus the rounding of the scale, 15 x 2^-11 of a step).  Rows outside the pool are skipped; rows of one call
+    must be distinct."""
+    _require_cuda(k=k)
+    _check_kv_rows(k, v)
+    if k.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"Expected dtype torch.float16 or torch.bfloat16, got {k.dtype}")
+    T, Hkv, D = k.shape
+    _check_vector("slot_mapping", slot_mapping, T, k.device)
+    _check_int4_pool(kv_pages, Hkv, D, page_size, k.device)
+    (k, k_tok, k_head), (v, v_tok, v_head) = _rows(k), _rows(v)
+    st = N.launch(k.device, N.lib().tb200_int4_cache_append, k.data_ptr(), v.data_ptr(), slot_mapping.data_ptr(),
+                  kv_pages.data_ptr(), N.dtype_code(k.dtype), T, Hkv, D, page_size, kv_pages.shape[0] * page_size,
+                  k_tok, k_head, v_tok, v_head)
+    N.check(st, "tb200_int4_cache_append")
+
+
+def int4_cache_gather(kv_pages: torch.Tensor, block_table: torch.Tensor, cu_seqlens_kv: torch.Tensor, total_tokens: int, *,
+                      dim: int, page_size: int, dtype: torch.dtype, cache_seqlens: Optional[torch.Tensor] = None,
+                      cu_seqlens_new: Optional[torch.Tensor] = None, k_new: Optional[torch.Tensor] = None,
+                      v_new: Optional[torch.Tensor] = None,
+                      out: "Optional[Tuple[torch.Tensor, torch.Tensor]]" = None) -> "Tuple[torch.Tensor, torch.Tensor]":
+    """Reads the 4-bit pool back: rows ``cu_seqlens_kv[b] .. cu_seqlens_kv[b + 1]`` of the returned K and V
+    ``[total_tokens,Hkv,dim]`` are request b's tokens 0, 1, ... in ``dtype``.  ``total_tokens`` may be an upper bound; rows
+    behind ``cu_seqlens_kv[-1]`` are left as they were (uninitialised in a new tensor).
+
+    With ``cache_seqlens``, ``cu_seqlens_new``, ``k_new`` and ``v_new`` only the first ``cache_seqlens[b]`` rows of a request
+    come from the cache and the rest from rows ``cu_seqlens_new[b] ..`` of ``k_new`` / ``v_new``."""
+    _require_cuda(kv_pages=kv_pages)
+    if kv_pages.dim() != 3:
+        raise ValueError(f"kv_pages must be [pages, heads_kv, page bytes], got {tuple(kv_pages.shape)}")
+    if dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"Expected dtype torch.float16 or torch.bfloat16, got {dtype}")
+    device, Hkv, total = kv_pages.device, kv_pages.shape[1], int(total_tokens)
+    _check_int4_pool(kv_pages, Hkv, dim, page_size, device)
+    batch = block_table.shape[0]
+    _check_table(block_table, batch, device)
+    _check_vector("cu_seqlens_kv", cu_seqlens_kv, batch + 1, device)
+    if total < 0:
+        raise ValueError("total_tokens must not be negative")
+    if cache_seqlens is not None:
+        if cu_seqlens_new is None or k_new is None or v_new is None:
+            raise ValueError("cache_seqlens, cu_seqlens_new, k_new and v_new come together")
+        _check_vector("cache_seqlens", cache_seqlens, batch, device)
+        _check_vector("cu_seqlens_new", cu_seqlens_new, batch + 1, device)
+        _check_kv_rows(k_new, v_new)
+        if tuple(k_new.shape[1:]) != (Hkv, dim) or k_new.dtype != dtype or k_new.device != device:
+            raise ValueError(f"k_new and v_new must be [tokens, {Hkv}, {dim}] with dtype {dtype} on {device}")
+        k_new, v_new = (t if t.is_contiguous() and t.data_ptr() % 16 == 0
+                        else t.clone(memory_format=torch.contiguous_format) for t in (k_new, v_new))
+    if out is None:
+        out = tuple(torch.empty((total, Hkv, dim), dtype=dtype, device=device) for _ in range(2))
+    for t in out:
+        if tuple(t.shape) != (total, Hkv, dim) or t.dtype != dtype or t.device != device or not t.is_contiguous():
+            raise ValueError(f"out must be two contiguous [{total}, {Hkv}, {dim}] tensors with dtype {dtype} on {device}")
+    st = N.launch(device, N.lib().tb200_int4_cache_gather, kv_pages.data_ptr(), block_table.data_ptr(),
+                  block_table.stride(0), block_table.shape[1], cu_seqlens_kv.data_ptr(), N.ptr(cache_seqlens),
+                  N.ptr(cu_seqlens_new), N.ptr(k_new), N.ptr(v_new), out[0].data_ptr(), out[1].data_ptr(),
+                  N.dtype_code(dtype), total, batch, Hkv, dim, page_size, kv_pages.shape[0])
+    N.check(st, "tb200_int4_cache_gather")
+    return out
+
+
+def _decode_int4_workspace(device: torch.device, batch: int, heads: int, heads_kv: int, dim: int) -> torch.Tensor:
+    """Scratch of the 4-bit decode.  Eager calls keep one buffer per (device, stream, shape), as the other decode calls do.
+    A call under capture gets one of its own from the graph's pool, cleared by a node of the graph: two graphs, or a
+    graph and an eager call, that run at the same time then never share counters."""
+    capturing = torch.cuda.is_current_stream_capturing()
+    key = (device, torch._C._cuda_getCurrentRawStream(device.index), "decode", batch, heads, heads_kv, dim, "int4")
+    ws = None if capturing else _WORKSPACES.get(key)
+    if ws is None:
+        need = N.lib().tb200_gqa_decode_int4_workspace_bytes(batch, heads, heads_kv, dim)
+        if need == 0:
+            raise ValueError("invalid decode problem size")
+        ws = torch.empty(need, dtype=torch.uint8, device=device)
+        ws[:(batch * heads + 8) * 4].zero_()            # TB200_DECODE_INT4_ZERO_BYTES
+        if not capturing:
+            _WORKSPACES[key] = ws
+    return ws
+
+
+def gqa_decode_int4(q: torch.Tensor, kv_pages: torch.Tensor, real_seqlen_kv: torch.Tensor, block_table: torch.Tensor, *,
+                    page_size: int, sm_scale: Optional[float] = None, softcap: float = 0.0,
+                    out_dtype: Optional[torch.dtype] = None, return_lse: bool = False, config: Optional[dict] = None):
+    """Single-token GQA decode over the 4-bit paged cache: q ``[B,H,D]``, ``kv_pages`` uint8
+    ``[pages,Hkv,page_size*(D+8)]``, ``real_seqlen_kv [B]`` and ``block_table [B,W]`` int32 -> o ``[B,H,D]`` (and the
+    log2-domain LSE ``[B,H]`` fp32).  An empty sequence gives zeros (LSE -inf); a page id outside the pool or a length
+    beyond the table makes that sequence NaN."""
+    _require_cuda(q=q)
+    if q.dim() != 3:
+        raise ValueError(f"q must have shape [B, H, D], got {tuple(q.shape)}")
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"Expected dtype torch.float16 or torch.bfloat16, got {q.dtype}")
+    if kv_pages.dim() != 3:
+        raise ValueError(f"kv_pages must be [pages, heads_kv, page bytes], got {tuple(kv_pages.shape)}")
+    B, H, D = q.shape
+    device, Hkv = q.device, kv_pages.shape[1]
+    if Hkv == 0 or H % Hkv != 0:
+        raise ValueError("heads must be divisible by heads_kv")
+    _check_int4_pool(kv_pages, Hkv, D, page_size, device)
+    _check_vector("real_seqlen_kv", real_seqlen_kv, B, device)
+    _check_table(block_table, B, device)
+    if not q.is_contiguous() or q.data_ptr() % 16:
+        q = q.clone(memory_format=torch.contiguous_format)
+    out_dtype = q.dtype if out_dtype is None else out_dtype
+    o = torch.empty((B, H, D), dtype=out_dtype, device=device)
+    lse = torch.empty((B, H), dtype=torch.float32, device=device) if return_lse else None
+    if B == 0:
+        return (o, lse) if return_lse else o
+    ws = _decode_int4_workspace(device, B, H, Hkv, D)
+    st = N.launch(device, N.lib().tb200_gqa_decode_int4, q.data_ptr(), kv_pages.data_ptr(), o.data_ptr(), N.ptr(lse),
+                  real_seqlen_kv.data_ptr(), block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
+                  N.dtype_code(q.dtype), N.dtype_code(out_dtype), B, H, Hkv, D, page_size, kv_pages.shape[0],
+                  D ** -0.5 if sm_scale is None else float(sm_scale), float(softcap or 0.0), N.decode_flags(config),
+                  ws.data_ptr(), ws.numel())
+    N.check(st, "tb200_gqa_decode_int4")
+    return (o, lse) if return_lse else o
+
+
+def gqa_prefill_paged_int4_cache(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, kv_pages: torch.Tensor,
+                                 cu_seqlens_q: torch.Tensor, cache_seqlens: torch.Tensor, block_table: torch.Tensor,
+                                 max_seqlen_q: int, *, page_size: int, is_causal: bool = True,
+                                 sm_scale: Optional[float] = None, softcap: float = 0.0) -> torch.Tensor:
+    """Packed prefill of one chunk per request over the 4-bit paged cache, appending the chunk: the cached tokens are read
+    back as packed 16-bit K/V next to the chunk's own rows, the packed prefill runs on it, and the chunk is quantised into
+    the pages.  The packed buffer is sized by the capacity of the block table and kept per shape; nothing is read back from
+    the device."""
+    _require_cuda(q=q, k_new=k_new, v_new=v_new, kv_pages=kv_pages)
+    total_q, H, D = q.shape
+    Hkv, B, device = k_new.shape[1], cu_seqlens_q.numel() - 1, q.device
+    if total_q == 0:
+        return torch.empty_like(q)
+    new_lens = cu_seqlens_q[1:] - cu_seqlens_q[:-1]
+    cu_kv = torch.zeros(B + 1, dtype=torch.int32, device=device)
+    cu_kv[1:] = torch.cumsum(cache_seqlens + new_lens, 0)
+    slots = paged_kv_plan(cache_seqlens, new_lens, block_table, None, None, total_q, page_size=page_size).slot_mapping
+    total_kv = B * block_table.shape[1] * int(page_size)
+    key = (device, torch.cuda.current_stream(device).cuda_stream, "int4_cache_packed", total_kv, Hkv, D, q.dtype)
+    capturing = torch.cuda.is_current_stream_capturing()
+    bufs = None if capturing else _WORKSPACES.get(key)
+    if bufs is None:
+        bufs = tuple(torch.empty((total_kv, Hkv, D), dtype=q.dtype, device=device) for _ in range(2))
+        if not capturing:
+            _WORKSPACES[key] = bufs
+    k_all, v_all = int4_cache_gather(kv_pages, block_table, cu_kv, total_kv, dim=D, page_size=page_size, dtype=q.dtype,
+                                     cache_seqlens=cache_seqlens, cu_seqlens_new=cu_seqlens_q, k_new=k_new, v_new=v_new,
+                                     out=bufs)
+    o = gqa_prefill_paged(q, k_all, v_all, None, None, cu_seqlens_q, None, None, int(max_seqlen_q), is_causal=is_causal,
+                          sm_scale=sm_scale, softcap=softcap, cu_seqlens_kv=cu_kv)
+    int4_cache_append(k_new, v_new, slots, kv_pages, page_size=page_size)
+    return o

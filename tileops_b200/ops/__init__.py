@@ -1,9 +1,11 @@
 from .gqa import (
     GroupedQueryAttentionDecodePagedFp8KVCacheFwdOp,
+    GroupedQueryAttentionDecodePagedInt4KVCacheFwdOp,
     GroupedQueryAttentionDecodePagedWithKVCacheFwdOp,
     GroupedQueryAttentionDecodeWithKVCacheFwdOp,
     GroupedQueryAttentionFwdOp,
     GroupedQueryAttentionPrefillFwdOp,
+    GroupedQueryAttentionPrefillPagedInt4KVCacheFwdOp,
     GroupedQueryAttentionPrefillPagedWithKVCacheFwdOp,
     GroupedQueryAttentionPrefillVarlenFwdOp,
     GroupedQueryAttentionSlidingWindowFwdOp,
@@ -11,6 +13,15 @@ from .gqa import (
 )
 from .mha import MultiHeadAttentionDecodePagedWithKVCacheFwdOp, MultiHeadAttentionDecodeWithKVCacheFwdOp
 from .op_base import Op
+from .paged_kv import (
+    Int4KVCacheAppendFwdOp,
+    Int4KVCacheGatherFwdOp,
+    PagedKVCachePlanFwdOp,
+    PagedKVCacheReleaseFwdOp,
+    QKNormRopeFwdOp,
+    QKNormRopeInt4KVCacheAppendFwdOp,
+    QKNormRopeKVCacheAppendFwdOp,
+)
 
 __all__ = [
     "Op",
@@ -25,4 +36,13 @@ __all__ = [
     "GroupedQueryAttentionDecodePagedFp8KVCacheFwdOp",
     "MultiHeadAttentionDecodeWithKVCacheFwdOp",
     "MultiHeadAttentionDecodePagedWithKVCacheFwdOp",
+    "GroupedQueryAttentionDecodePagedInt4KVCacheFwdOp",
+    "GroupedQueryAttentionPrefillPagedInt4KVCacheFwdOp",
+    "PagedKVCachePlanFwdOp",
+    "PagedKVCacheReleaseFwdOp",
+    "QKNormRopeFwdOp",
+    "QKNormRopeKVCacheAppendFwdOp",
+    "QKNormRopeInt4KVCacheAppendFwdOp",
+    "Int4KVCacheAppendFwdOp",
+    "Int4KVCacheGatherFwdOp",
 ]

@@ -13,7 +13,10 @@ against the reference runs unchanged; only the kernels behind the ``kernel_map``
 * prefill ops take ``return_lse=True`` to also return the log2-domain LSE ``[B, H, Sq]`` that
   the reference kernels compute and drop (``kernels/attention/gqa_fwd.py:573``);
 * ``GroupedQueryAttentionDecodePagedFp8KVCacheFwdOp`` is an addition (FP8-e4m3 cache with one
-  fp32 scale per (page, KV head)).
+  fp32 scale per (page, KV head));
+* ``GroupedQueryAttentionDecodePagedInt4KVCacheFwdOp`` and
+  ``GroupedQueryAttentionPrefillPagedInt4KVCacheFwdOp`` are additions (cache held in 4 bits with one
+  float16 scale and offset per token and KV head; its writers are in ``ops/paged_kv.py``).
 """
 
 from __future__ import annotations
@@ -24,9 +27,11 @@ import torch
 
 from ..kernels import (
     GQADecodePagedFp8Sm100Kernel,
+    GQADecodePagedInt4Sm100Kernel,
     GQADecodePagedSm100Kernel,
     GQADecodeSm100Kernel,
     GQAPrefillPagedFp8CacheSm100Kernel,
+    GQAPrefillPagedInt4CacheSm100Kernel,
     GQAPrefillPagedRopeSm100Kernel,
     GQAPrefillPagedSm100Kernel,
     GQAPrefillSm100Kernel,
@@ -58,6 +63,8 @@ __all__ = [
     "GroupedQueryAttentionDecodeWithKVCacheFwdOp",
     "GroupedQueryAttentionDecodePagedWithKVCacheFwdOp",
     "GroupedQueryAttentionDecodePagedFp8KVCacheFwdOp",
+    "GroupedQueryAttentionDecodePagedInt4KVCacheFwdOp",
+    "GroupedQueryAttentionPrefillPagedInt4KVCacheFwdOp",
 ]
 
 
@@ -851,12 +858,15 @@ class GroupedQueryAttentionDecodePagedWithKVCacheFwdOp(Op):
     _KEYS = PAGED_DECODE_KEYS
     validate_inputs = False
 
+    def _pool_pages(self, k: torch.Tensor) -> int:
+        return k.shape[0] // self.page_size
+
     def _check_table(self, k: torch.Tensor, real_seqlen_kv: torch.Tensor, block_table: torch.Tensor) -> None:
         """Host-side range check of lengths and the page ids they reach (synchronises)."""
         lens = real_seqlen_kv.detach().cpu().to(torch.int64)
         table = block_table.detach().cpu().to(torch.int64)
         width = table.shape[1]
-        pool_pages = k.shape[0] // self.page_size
+        pool_pages = self._pool_pages(k)
         if bool((lens < 0).any()):
             raise ValueError("real_seqlen_kv must be non-negative")
         need = (lens + self.page_size - 1) // self.page_size
@@ -942,3 +952,151 @@ class GroupedQueryAttentionDecodePagedFp8KVCacheFwdOp(GroupedQueryAttentionDecod
         data = dict(vars(self))
         data["dtype"] = getattr(self, "cache_dtype", None) or fp8_dtype()
         return gqa_decode_paged_roofline(data)
+
+
+def _check_int4_pool_shape(kv_pages, heads_kv: int, page_size: int, dim: int, pages: Optional[int] = None) -> None:
+    want = (heads_kv, page_size * (dim + 8))
+    if kv_pages.ndim != 3 or tuple(kv_pages.shape[1:]) != want or pages not in (None, kv_pages.shape[0]):
+        raise ValueError(f"kv_pages must have shape [{'pages' if pages is None else pages}, {want[0]}, {want[1]}], "
+                         f"got {tuple(kv_pages.shape)}")
+
+
+class GroupedQueryAttentionDecodePagedInt4KVCacheFwdOp(GroupedQueryAttentionDecodePagedWithKVCacheFwdOp):
+    """Paged decode over a cache held in 4 bits: ``forward(q, kv_pages, real_seqlen_kv, block_table)`` with the pool that
+    :class:`~tileops_b200.ops.Int4KVCacheAppendFwdOp` writes, uint8 ``[seqlen_kv / page_size, heads_kv, page_size * (dim +
+    8)]``.  Matches dequantise-then-attend.  An empty sequence gives zeros; a page id outside the pool, or a length beyond
+    the table, makes that sequence's output NaN (nothing outside the pool is read)."""
+
+    _KEYS = ("gqa_decode_paged_int4_kernel",)
+
+    def __init__(self, batch: int, heads: int, heads_kv: int, seqlen_kv: int, dim: int, page_size: int,
+                 sm_scale: Optional[float] = None, softcap: Optional[float] = None,
+                 kernel_map: Optional[Dict[str, type]] = None, tune: bool = False) -> None:
+        super().__init__(batch, heads, heads_kv, seqlen_kv, dim, page_size, sm_scale, softcap, kernel_map, tune)
+        self._by_dtype: dict = {}
+
+    @property
+    def default_kernel_map(self) -> Dict[str, type]:
+        return {"gqa_decode_paged_int4_kernel": GQADecodePagedInt4Sm100Kernel}
+
+    def _infer_output_shapes(self, q_shape, *rest) -> Dict[str, tuple]:
+        return {"o": tuple(q_shape)}
+
+    def forward(self, q, kv_pages, real_seqlen_kv, block_table) -> torch.Tensor:
+        if tuple(q.shape) != (self.batch, self.heads, self.dim):
+            raise ValueError(f"q must have shape {(self.batch, self.heads, self.dim)}, got {tuple(q.shape)}")
+        _check_int4_pool_shape(kv_pages, self.heads_kv, self.page_size, self.dim, self.seqlen_kv // self.page_size)
+        self.dtype = q.dtype
+        if self.validate_inputs:
+            self._check_table(kv_pages, real_seqlen_kv, block_table)
+        inputs = (q, kv_pages, real_seqlen_kv, block_table)
+        if self._builder is None and q.dtype in self._by_dtype:     # selected before, in tree
+            return self._by_dtype[q.dtype](*inputs)
+        kernel = self._get_kernel(inputs, q.dtype)
+        if self._builder is None:
+            self._by_dtype[q.dtype] = kernel
+        return kernel(*inputs)
+
+    def _pool_pages(self, kv_pages) -> int:
+        return kv_pages.shape[0]
+
+    def eval_roofline(self) -> tuple:
+        from ..perf.formulas import gqa_decode_paged_int4_roofline
+        return gqa_decode_paged_int4_roofline(self)
+
+
+class GroupedQueryAttentionPrefillPagedInt4KVCacheFwdOp(Op):
+    """Packed GQA prefill of one chunk per request over a paged cache held in 4 bits, with the append (THD).
+
+    ``forward(q, k_new, v_new, kv_pages, cu_seqlens_q, cache_seqlens, block_table, max_seqlen_q)``: request b attends to
+    its ``cache_seqlens[b]`` cached tokens (read back from ``kv_pages``) followed by its own rows of ``k_new`` / ``v_new``
+    (as they are), and the chunk is quantised into ``kv_pages`` in place, as
+    :class:`GroupedQueryAttentionPrefillPagedWithKVCacheFwdOp` does for its e4m3 cache.  Lengths and page ids are range
+    checked on the host, as there; ``validate_inputs = False`` on an instance leaves that out (and with it the reads of
+    the device)."""
+
+    validate_inputs = True
+
+    def __init__(self, batch: int, heads: int, heads_kv: int, max_pages_per_req: int, page_size: int, dim: int,
+                 is_causal: bool = True, sm_scale: Optional[float] = None, softcap: Optional[float] = None,
+                 kernel_map: Optional[Dict[str, type]] = None, tune: bool = False) -> None:
+        _validate_gqa_dims(heads, heads_kv, dim)
+        _validate_positive(batch=batch, max_pages_per_req=max_pages_per_req, page_size=page_size)
+        self.batch, self.heads, self.heads_kv, self.dim = batch, heads, heads_kv, dim
+        self.max_pages_per_req, self.page_size = max_pages_per_req, page_size
+        self.max_cache_len = max_pages_per_req * page_size
+        self.is_causal = is_causal
+        self.sm_scale = _attention_scale(dim, sm_scale)
+        self.softcap = _score_softcap(softcap)
+        self.tune = tune
+        self.dispatch_kernel(kernel_map)
+
+    @property
+    def default_kernel_map(self) -> Dict[str, type]:
+        return {"gqa_prefill_paged_with_int4_kv_cache_fwd_kernel": GQAPrefillPagedInt4CacheSm100Kernel}
+
+    def attention_call(self, dtype: torch.dtype) -> AttentionCall:
+        return AttentionCall(
+            dtype=dtype, batch=self.batch, heads=self.heads, heads_kv=self.heads_kv, dim=self.dim,
+            max_pages_per_req=self.max_pages_per_req, page_size=self.page_size, is_causal=self.is_causal,
+            sm_scale=self.sm_scale, softcap=self.softcap, tune=self.tune)
+
+    def _infer_output_shapes(self, q_shape, *rest) -> Dict[str, tuple]:
+        return {"o": tuple(q_shape)}
+
+    def _check_forward_inputs(self, q, k_new, v_new, kv_pages, cu_seqlens_q, cache_seqlens, block_table) -> None:
+        for name, t in (("q", q), ("k_new", k_new), ("v_new", v_new), ("kv_pages", kv_pages),
+                        ("cu_seqlens_q", cu_seqlens_q), ("cache_seqlens", cache_seqlens), ("block_table", block_table)):
+            if t.device.type != "cuda":
+                raise ValueError(f"{name} must be on a cuda device, got {t.device}")
+            if t.device != q.device:
+                raise ValueError(f"{name} must be on {q.device}, got {t.device}")
+        _validate_attention_dtype(q.dtype)
+        if q.ndim != 3 or tuple(q.shape[1:]) != (self.heads, self.dim):
+            raise ValueError(f"q must have shape [total_q, {self.heads}, {self.dim}], got {tuple(q.shape)}")
+        for name, t in (("k_new", k_new), ("v_new", v_new)):
+            if tuple(t.shape) != (q.shape[0], self.heads_kv, self.dim) or t.dtype != q.dtype:
+                raise ValueError(f"{name} must be {q.dtype} with shape {(q.shape[0], self.heads_kv, self.dim)}, "
+                                 f"got {t.dtype} {tuple(t.shape)}")
+        _check_int4_pool_shape(kv_pages, self.heads_kv, self.page_size, self.dim)
+        for name, t, shape in (("cu_seqlens_q", cu_seqlens_q, (self.batch + 1,)), ("cache_seqlens", cache_seqlens, (self.batch,)),
+                               ("block_table", block_table, (self.batch, self.max_pages_per_req))):
+            if t.dtype != torch.int32 or tuple(t.shape) != shape:
+                raise ValueError(f"{name} must be torch.int32 with shape {shape}, got {t.dtype} {tuple(t.shape)}")
+
+    def _check_ranges(self, q, kv_pages, cu_seqlens_q, cache_seqlens, block_table, max_seqlen_q: int) -> None:
+        """Host-side range checks (one copy back, synchronises)."""
+        cu, cached = cu_seqlens_q.cpu().long(), cache_seqlens.cpu().long()
+        new = cu[1:] - cu[:-1]
+        if int(cu[0]) != 0 or bool((new < 0).any()):
+            raise ValueError("cu_seqlens_q must start at 0 and be non-decreasing")
+        if int(cu[-1]) != q.shape[0]:
+            raise ValueError(f"cu_seqlens_q[-1] ({int(cu[-1])}) must equal q.shape[0] ({q.shape[0]})")
+        if max_seqlen_q < int(new.max()):
+            raise ValueError(f"max_seqlen_q ({max_seqlen_q}) must be >= actual max Q sequence length ({int(new.max())})")
+        if bool((cached < 0).any()):
+            raise ValueError("cache_seqlens must be non-negative")
+        total = cached + new
+        if int(total.max()) > self.max_cache_len:
+            raise ValueError("cache_seqlens + q_len exceeds paged KV capacity: "
+                             f"max total length {int(total.max())}, capacity {self.max_cache_len}")
+        table = block_table.cpu().long()
+        live = torch.arange(table.shape[1])[None] < ((total + self.page_size - 1) // self.page_size)[:, None]
+        bad = live & ((table < 0) | (table >= kv_pages.shape[0]))
+        if bool(bad.any()):
+            b, i = (int(x) for x in bad.nonzero()[0])
+            raise ValueError(f"block_table[{b}, {i}]={int(table[b, i])} is outside the pool of {kv_pages.shape[0]} pages")
+
+    def forward(self, q, k_new, v_new, kv_pages, cu_seqlens_q, cache_seqlens, block_table, max_seqlen_q) -> torch.Tensor:
+        self._check_forward_inputs(q, k_new, v_new, kv_pages, cu_seqlens_q, cache_seqlens, block_table)
+        if self.validate_inputs:
+            self._check_ranges(q, kv_pages, cu_seqlens_q, cache_seqlens, block_table, int(max_seqlen_q))
+        self.dtype = q.dtype
+        call = self.attention_call(q.dtype)
+        key = self.select_kernel_key(("gqa_prefill_paged_with_int4_kv_cache_fwd_kernel",), call)
+        inputs = (q, k_new, v_new, kv_pages, cu_seqlens_q, cache_seqlens, block_table)
+        kernel = self.get_or_build_kernel(key, inputs, key=call.dtype, build=lambda: self.kernel_map[key](
+            batch=call.batch, heads=call.heads, heads_kv=call.heads_kv, max_pages_per_req=call.max_pages_per_req,
+            page_size=call.page_size, dim=call.dim, is_causal=call.is_causal, dtype=call.dtype, sm_scale=call.sm_scale,
+            softcap=call.softcap, tune=call.tune))
+        return kernel(*inputs, int(max_seqlen_q))

@@ -175,3 +175,14 @@ def gqa_decode_paged_roofline(op: Any = None, **kwargs: Any) -> tuple:
     kv_elems = seqlen_kv * heads_kv * dim
     meta = batch * 4 + batch * max(1, -(-seqlen_kv // page)) * 4
     return int(4 * batch * heads * seqlen_kv * dim), int((2 * q_elems + 2 * kv_elems) * e + meta)
+
+
+def gqa_decode_paged_int4_roofline(op: Any = None, **kwargs: Any) -> tuple:
+    """Paged decode over a 4-bit cache: per token and KV head ``dim`` bytes of codes (K and V) and 8 of parameters;
+    ``seqlen_kv`` is the pool size in tokens, as in the other paged decode formulas."""
+    d = _fields(op, kwargs)
+    batch, heads, heads_kv, seqlen_kv, dim = (int(d[k]) for k in ("batch", "heads", "heads_kv", "seqlen_kv", "dim"))
+    page = int(d["page_size"])
+    meta = batch * 4 + batch * max(1, -(-seqlen_kv // page)) * 4
+    return (int(4 * batch * heads * seqlen_kv * dim),
+            int(2 * batch * heads * dim * _itemsize(_dtype_of(d)) + seqlen_kv * heads_kv * (dim + 8) + meta))
