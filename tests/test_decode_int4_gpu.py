@@ -3,8 +3,9 @@
 Tolerance of the decode with an fp32 output, per (sequence, KV head), from the arithmetic the kernel may use:
   * P times the V scale is rounded to float16 before it meets the codes (0..15): 2^-11 * 15 max|vs|;
   * a score is a sum of D products accumulated in fp32 and scaled: off by at most 2^-19 A, A = scale * sum|q| *
-    max(15 |ks| + |km|); with a softcap the capped score is off by 2^-20 cap more; probabilities move by as much
-    (relative) and the output by at most twice that times max|v|;
+    max(15 |ks| + |km|); a q below 2^-6 of its head's largest may be rounded to an integer of a scale where that is
+    2^13 or more, which adds scale * 15 max|ks| * 2^-14 max|q| for each such value; with a softcap the capped score is off by
+    2^-20 cap more; probabilities move by as much (relative) and the output by at most twice that times max|v|;
   * the row sums and the exponentials: 2^-16 max|v| at the lengths used here.
 A 16-bit output adds half a step of its type.  The LSE is off by the score's error, 2^-16 and the rounding of its value.
 """
@@ -68,7 +69,9 @@ def tolerances(q, pages, lens, table, page, scale, softcap):
         for h in range(H):
             hk = h // (H // Hkv)
             A = scale * float(q[b, h].double().abs().sum()) * float((15 * a[:, hk, 0] + a[:, hk, 1]).max())
-            score = 2.0 ** -19 * A + 2.0 ** -20 * softcap
+            x = q[b, h].double().abs()
+            small = float((x < 2.0 ** -6 * x.max()).sum()) * 2.0 ** -14 * float(x.max())
+            score = 2.0 ** -19 * A + scale * 15 * float(a[:, hk, 0].max()) * small + 2.0 ** -20 * softcap
             vmax = float(v[:, hk].abs().max())
             to[b, h] = 2.0 ** -11 * 15 * float(a[:, hk, 2].max()) + 2 * score * vmax + 2.0 ** -16 * vmax
             tl[b, h] = 1.4427 * score + 2.0 ** -16
@@ -347,3 +350,19 @@ def test_prefill_reads_the_cache_as_gather_does_and_appends_as_append_does():
     cu_kv = i32([0, total[0], total[0] + total[1], sum(total)])
     ref = F.gqa_prefill_paged(q, k_all, v_all, None, None, cu, None, None, 40, cu_seqlens_kv=cu_kv)
     assert torch.equal(o, ref)
+
+
+@pytest.mark.parametrize("chunk", [1, 2, 3, 7])
+@pytest.mark.parametrize("H,D,page", [(8, 128, 16), (8, 64, 128), (32, 128, 128), (24, 64, 48)])
+def test_fixed_runs_agree_with_the_partition_the_kernel_picks(H, D, page, chunk):
+    lens = [700, 3000, 0, 1, 2049, 128]
+    check(lens, H, 2, D, page, config={"chunk_tiles": chunk}, seed=chunk)
+
+
+def test_many_short_segments_per_block_are_bit_reproducible():
+    q, pages, lens, table = make([2000, 1333, 128, 999] * 16, 16, 4, 128, 64, seed=14)
+    for chunk in (1, 2, 5):
+        want = F.gqa_decode_int4(q, pages, lens, table, page_size=64, config={"chunk_tiles": chunk})
+        for _ in range(60):
+            assert torch.equal(F.gqa_decode_int4(q, pages, lens, table, page_size=64, config={"chunk_tiles": chunk}), want)
+    assert F.decode_status() == 0
