@@ -64,11 +64,17 @@ constexpr uint32_t kMid = 0x47804780u;   // 7.5 twice in float16
 #ifndef TB200_INT4_B128
 #define TB200_INT4_B128 3
 #endif
+#ifndef TB200_INT4_MINRUN
+#define TB200_INT4_MINRUN 4
+#endif
+#ifndef TB200_INT4_B2_64
+#define TB200_INT4_B2_64 2
+#endif
 #ifndef TB200_INT4_R64
-#define TB200_INT4_R64 2
+#define TB200_INT4_R64 4
 #endif
 #ifndef TB200_INT4_S64
-#define TB200_INT4_S64 6
+#define TB200_INT4_S64 3
 #endif
 #ifndef TB200_INT4_B64
 #define TB200_INT4_B64 3
@@ -102,7 +108,7 @@ struct Cfg {
   static constexpr int kTile = kRecords * kInt4Tokens;                        // tokens per tile
   static constexpr int kStageBytes = kRecords * kRec;
   static constexpr int kStages = D == 128 ? TB200_INT4_S128 : TB200_INT4_S64;
-  static constexpr int kBlocks = NT == 2 ? 2 : D == 128 ? TB200_INT4_B128 : TB200_INT4_B64;   // blocks per SM
+  static constexpr int kBlocks = NT == 2 ? (D == 64 ? TB200_INT4_B2_64 : 2) : D == 128 ? TB200_INT4_B128 : TB200_INT4_B64;   // blocks per SM
   static constexpr int kHeads = 8 * NT;
   static constexpr int kQSlotBytes = kHeads * D * 2;
   static constexpr int kFrags = NT * D / 16;             // accumulator fragments of a warp
@@ -111,7 +117,8 @@ struct Cfg {
   static constexpr int dump = qslots + kItemSlots * kQSlotBytes;              // [kWarps][kFrags][32] float4
   static constexpr int ml = dump + kWarps * kFrags * 512;                     // [kWarps][NT][4] float4
   static constexpr int bars = ml + kWarps * NT * 64;
-  static constexpr int misc = bars + 8 * (2 * kStages + 2 * kItemSlots + 2);  // 16 ints
+  static constexpr int segs = bars + 8 * (2 * kStages + 2 * kItemSlots + 2);  // [kItemSlots] Segment
+  static constexpr int misc = segs + kItemSlots * 64;                         // 16 ints
   static constexpr int plan = misc + 64;                                      // s_prefix [batch + 1], s_lens [batch]
   static_assert(qslots % 128 == 0 && dump % 16 == 0 && bars % 8 == 0, "layout");
 };
@@ -122,13 +129,14 @@ size_t smem_bytes(int batch) {
 }
 
 // A segment: the tiles of one lane (sequence, KV head, head block) that one range of the partition covers.
-struct Segment {
+struct alignas(16) Segment {
   int b, hk, hbi, len;
-  int tile0, tile1;
-  int n_runs, first_range, slot, lane;
+  int tile0, tile1, n_runs, slot;
   unsigned lane_start, next;
-  bool too_long;
+  int first_range, lane;
+  int too_long;
 };
+static_assert(sizeof(Segment) <= 64, "a slot of shared memory");
 __device__ __forceinline__ Segment segment_at(const Int4DecodeParams& p, unsigned u, unsigned range_begin,
                                               unsigned range_end, int range, unsigned per, const int* s_prefix,
                                               const int* s_lens) {
@@ -147,7 +155,7 @@ __device__ __forceinline__ Segment segment_at(const Int4DecodeParams& p, unsigne
   const unsigned local = u - unsigned(s_prefix[lo]) * unsigned(lanes);
   const int rem = int(local / tiles_b);
   const unsigned t = local - unsigned(rem) * tiles_b;
-  g.hk = rem / p.n_hb;
+  g.hk = p.n_hb == 1 ? rem : rem / p.n_hb;
   g.hbi = rem - g.hk * p.n_hb;
   g.lane = lo * lanes + rem;
   g.lane_start = u - t;
@@ -155,8 +163,9 @@ __device__ __forceinline__ Segment segment_at(const Int4DecodeParams& p, unsigne
   g.next = min(range_end, lane_end);
   g.tile0 = int(t);
   g.tile1 = int(t + (g.next - u));
-  g.first_range = int(g.lane_start / per);
-  g.n_runs = int((lane_end - 1) / per) - g.first_range + 1;
+  const bool whole = g.lane_start >= range_begin && lane_end <= range_end;
+  g.first_range = whole ? range : int(g.lane_start / per);
+  g.n_runs = whole ? 1 : int((lane_end - 1) / per) - g.first_range + 1;
   g.slot = 2 * range + (u == range_begin ? 0 : 1);
   return g;
 }
@@ -367,28 +376,32 @@ __global__ void __launch_bounds__(kAllThreads, Cfg<D, NT>::kBlocks) gqa_decode_i
   if (warp < kWarps) tile_plan<C::kTile>(p, tid, s_prefix, s_lens, s_misc + 2, s_misc + 8);
   __syncthreads();
 
-  // Units (tiles) per range.  An equal share per block, or, for a batch of equal lengths, lanes cut into equal parts.
+  // Units (tiles) per range: an equal share per block, but no run shorter than kMinRun tiles (a run costs its partial
+  // result's way through memory, and the merge of a lane reads all of them).  Sequences of equal length are cut at whole
+  // lanes, or at equal parts of lanes, where that leaves the blocks busy to within a twentieth: fewer runs to merge.
   const unsigned lanes = unsigned(p.heads_kv) * unsigned(p.n_hb);
   const unsigned total_units = unsigned(s_prefix[p.batch]) * lanes;
-  unsigned per = max((total_units + gridDim.x - 1) / gridDim.x, 1u);
-  bool split = true;     // whether a lane may be shared by ranges (and need slots for partial results)
+  unsigned per = max((total_units + gridDim.x - 1) / gridDim.x, unsigned(TB200_INT4_MINRUN));
   if (p.force_chunk > 0) {
-    per = unsigned(p.force_chunk);
-  } else if (!(s_misc[8] | s_misc[9] | s_misc[10] | s_misc[11]) && total_units > 0 && per < 256u) {
-    const unsigned L = unsigned(s_prefix[1]);
-    const unsigned lanes_total = unsigned(p.batch) * lanes;
-    constexpr unsigned kMinRun = 4;
-    unsigned k = 1;
-    while (k < 32u && 5u * lanes_total * k < 4u * gridDim.x && L % (2u * k) == 0u && L / (2u * k) >= kMinRun) k *= 2u;
-    const unsigned ranges = lanes_total * k, waves = (ranges + gridDim.x - 1) / gridDim.x;
-    if (4u * ranges >= 3u * waves * gridDim.x || k == 32u || L / (2u * k) < kMinRun) {
-      per = L / k;
-      split = k > 1;
+    // never so short that the ranges outnumber the slots of the workspace (2 per range)
+    per = max(unsigned(p.force_chunk), (2u * total_units + unsigned(p.max_slots) - 1) / unsigned(p.max_slots));
+  } else if (!(s_misc[8] | s_misc[9] | s_misc[10] | s_misc[11]) && total_units > 0) {
+    const unsigned L = unsigned(s_prefix[1]), lanes_total = unsigned(p.batch) * lanes;
+    if (lanes_total >= gridDim.x) {
+      const unsigned whole = (lanes_total + gridDim.x - 1) / gridDim.x * L;
+      if (20ull * whole <= 21ull * per) per = whole;
+    } else if (L <= per) {
+      per = L;
+    } else {
+      for (unsigned k = (L + per - 1) / per, i = 0; k > 1 && i < 4; --k, ++i) {
+        const unsigned part = (L + k - 1) / k;
+        if (L % part == 0) {
+          if (20ull * part <= 21ull * per) per = part;
+          break;
+        }
+      }
     }
   }
-  // never so small that the ranges outnumber the slots of the workspace (2 per range)
-  if (split) per = max(per, (2u * total_units + unsigned(p.max_slots) - 1) / unsigned(p.max_slots));
-  const int n_ranges = int((total_units + per - 1) / per);
   const long long limit = p.wait_cycles;
 
   if (warp == kWarps) {
@@ -398,7 +411,7 @@ __global__ void __launch_bounds__(kAllThreads, Cfg<D, NT>::kBlocks) gqa_decode_i
     int stage = 0, round = 0;
     uint32_t stage_par = 0;
     bool alive = true;
-    for (int range = blockIdx.x; alive && range < n_ranges; range += gridDim.x) {
+    for (int range = blockIdx.x; alive && (unsigned long long)range * per < total_units; range += gridDim.x) {
       const unsigned range_begin = unsigned(range) * per, range_end = min(range_begin + per, total_units);
       for (unsigned u = range_begin; alive && u < range_end; ++round) {
         const int slot = round & 1;
@@ -409,6 +422,7 @@ __global__ void __launch_bounds__(kAllThreads, Cfg<D, NT>::kBlocks) gqa_decode_i
         const Segment d = segment_at(p, u, range_begin, range_end, range, per, s_prefix, s_lens);
         u = d.next;
         if (lane == 0) {
+          *reinterpret_cast<Segment*>(smem + C::segs + slot * 64) = d;     // the math warps need not work it out again
           const int head0 = d.hk * p.group + d.hbi * p.hb;
           const uint32_t q_bytes = uint32_t(min(p.hb, p.group - d.hbi * p.hb)) * D * 2;
           mbar_expect_tx(bar_item_full(slot), q_bytes);
@@ -495,14 +509,14 @@ __global__ void __launch_bounds__(kAllThreads, Cfg<D, NT>::kBlocks) gqa_decode_i
 
     int stage = 0, round = 0;
     uint32_t stage_par = 0;
-    for (int range = blockIdx.x; alive && range < n_ranges; range += gridDim.x) {
+    for (int range = blockIdx.x; alive && (unsigned long long)range * per < total_units; range += gridDim.x) {
       const unsigned range_begin = unsigned(range) * per, range_end = min(range_begin + per, total_units);
       unsigned last_begin = range_begin;     // first unit of the range's last segment
       for (unsigned u = range_begin; alive && u < range_end; ++round) {
         const int slot = round & 1;
         last_begin = u;
         if (!mbar_wait(bar_item_full(slot), (round >> 1) & 1, s_abort, status, 602, limit)) { alive = false; break; }
-        const Segment d = segment_at(p, u, range_begin, range_end, range, per, s_prefix, s_lens);
+        const Segment d = *reinterpret_cast<const Segment*>(smem + C::segs + slot * 64);
         u = d.next;
         const int head0 = d.hk * p.group + d.hbi * p.hb;
         const int n_heads = min(p.hb, p.group - d.hbi * p.hb);
@@ -819,17 +833,19 @@ __global__ void __launch_bounds__(kAllThreads, Cfg<D, NT>::kBlocks) gqa_decode_i
       const Segment last = one ? first : segment_at(p, last_begin, range_begin, range_end, range, per, s_prefix, s_lens);
       if (first.n_runs == 1 && last.n_runs == 1) continue;
       if (!wait_merged()) break;          // every warp's partial results are written
-      if (tid == 0) {
-        auto ticket = [&](const Segment& d) {
+      if (lane == 0 && warp < 2) {        // one thread takes the first segment's ticket, another the last one's
+        const Segment& d = warp == 0 ? first : last;
+        int mine = 0;
+        if (d.n_runs > 1 && (warp == 0 || !one)) {
           int* at = p.counters + kCounterWords + d.lane;
           int n;
           asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(n) : "l"(at) : "memory");
-          if (n != d.n_runs - 1) return 0;
-          *at = 0;      // zero again for the next launch
-          return 1;
-        };
-        s_misc[6] = first.n_runs > 1 ? ticket(first) : 0;
-        s_misc[7] = !one && last.n_runs > 1 ? ticket(last) : 0;
+          if (n == d.n_runs - 1) {
+            *at = 0;      // zero again for the next launch
+            mine = 1;
+          }
+        }
+        s_misc[6 + warp] = mine;
       }
       mbar_arrive(bar_dump);
       if (!wait_dump()) break;
@@ -840,10 +856,20 @@ __global__ void __launch_bounds__(kAllThreads, Cfg<D, NT>::kBlocks) gqa_decode_i
         for (int f = warp; f < C::kFrags; f += kWarps) {
           Merged a;
           merge_begin(a);
-#pragma unroll 4
-          for (int r = 0; r < d.n_runs; ++r) {
-            const size_t it = size_t(segment_slot(d.first_range + r, per, d.lane_start));
-            merge_add(a, __ldcg(p.part_o + (it * C::kFrags + f) * 32 + lane), __ldcg(p.part_ml + (it * NT + f / kKSteps) * 4 + t4));
+          // sixteen runs in flight: a long lane cut over all SMs has dozens, and their latency would add up
+          constexpr int kBatch = 16;
+          for (int r0 = 0; r0 < d.n_runs; r0 += kBatch) {
+            float4 o[kBatch], ml[kBatch];
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+              const int r = min(r0 + i, d.n_runs - 1);
+              const size_t it = size_t(segment_slot(d.first_range + r, per, d.lane_start));
+              o[i] = __ldcg(p.part_o + (it * C::kFrags + f) * 32 + lane);
+              ml[i] = __ldcg(p.part_ml + (it * NT + f / kKSteps) * 4 + t4);
+            }
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i)
+              if (r0 + i < d.n_runs) merge_add(a, o[i], ml[i]);
           }
           emit<D, TO>(p, a, d.b, d.hk * p.group + d.hbi * p.hb, min(p.hb, p.group - d.hbi * p.hb), f, lane);
         }
