@@ -856,8 +856,8 @@ __global__ void __launch_bounds__(kAllThreads, Cfg<D, NT>::kBlocks) gqa_decode_i
         for (int f = warp; f < C::kFrags; f += kWarps) {
           Merged a;
           merge_begin(a);
-          // sixteen runs in flight: a long lane cut over all SMs has dozens, and their latency would add up
-          constexpr int kBatch = 16;
+          // ten runs in flight: a long lane cut over all SMs has dozens, and their latency would add up
+          constexpr int kBatch = 10;
           for (int r0 = 0; r0 < d.n_runs; r0 += kBatch) {
             float4 o[kBatch], ml[kBatch];
 #pragma unroll

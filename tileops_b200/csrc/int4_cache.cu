@@ -20,52 +20,93 @@ struct GatherParams {
   int batch, heads_kv, page_size, table_width, pool_pages, total;
 };
 
-// One block per output token.  kLanes lanes hold a row, 8 values each.
+// A block of kTokens consecutive output rows (tokens).  One thread per token finds where it comes from (a binary search and
+// a block-table entry); then D / 16 lanes expand a row of one token and KV head, 16 values each, and neighbouring groups
+// take neighbouring tokens, whose rows lie next to each other in a record.  kAhead rows are requested before the first is
+// expanded.
+constexpr int kTokens = 32;
+constexpr int kAhead = 4;
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) int4_gather_kernel(GatherParams p) {
-  constexpr int kLanes = D / 8;
-  const int g = blockIdx.x;
-  if (g < p.cu[0] || g >= p.cu[p.batch]) return;   // `total` may be an upper bound: the host never reads the lengths
-  int lo = 0, hi = p.batch - 1;     // largest b with cu[b] <= g
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (p.cu[mid] <= g) lo = mid; else hi = mid - 1;
-  }
-  const int t = g - p.cu[lo];
-  const int lane = threadIdx.x % kLanes;
-  if (p.cached && t >= p.cached[lo]) {
-    const size_t src = size_t(p.cu_new[lo] + t - p.cached[lo]) * p.heads_kv * D;
-    for (int i = threadIdx.x * 8; i < p.heads_kv * D; i += kThreads * 8) {
-      *reinterpret_cast<uint4*>(static_cast<T*>(p.k_out) + size_t(g) * p.heads_kv * D + i) =
-          *reinterpret_cast<const uint4*>(static_cast<const T*>(p.k_new) + src + i);
-      *reinterpret_cast<uint4*>(static_cast<T*>(p.v_out) + size_t(g) * p.heads_kv * D + i) =
-          *reinterpret_cast<const uint4*>(static_cast<const T*>(p.v_new) + src + i);
+  constexpr int kLanes = D / 16;
+  constexpr int kGroups = kThreads / kLanes;
+  __shared__ long long s_src[kTokens];    // >= 0: byte of the token's K codes in its record, of head 0; -1: NaN; -2: nothing;
+                                          // <= -3: row -(src + 3) of k_new / v_new
+  const int g0 = blockIdx.x * kTokens;
+  const long long head_bytes = (long long)(p.page_size / kInt4Tokens) * int4_record_bytes(D);
+  if (g0 >= p.cu[p.batch]) return;        // `total` may be an upper bound: the host never reads the lengths
+  if (threadIdx.x < kTokens) {
+    const int g = g0 + threadIdx.x;
+    long long src = -2;
+    if (g < p.total && g >= p.cu[0] && g < p.cu[p.batch]) {
+      int lo = 0, hi = p.batch - 1;       // largest b with cu[b] <= g
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (p.cu[mid] <= g) lo = mid; else hi = mid - 1;
+      }
+      const int t = g - p.cu[lo];
+      if (p.cached && t >= p.cached[lo]) {
+        src = -3 - ((long long)p.cu_new[lo] + t - p.cached[lo]);
+      } else {
+        const int column = t / p.page_size, off = t - column * p.page_size;
+        const int page = column < p.table_width ? p.table[int64_t(lo) * p.table_stride + column] : -1;
+        src = page >= 0 && page < p.pool_pages      // a page outside the pool reads as NaN
+                  ? (long long)page * p.heads_kv * head_bytes + (long long)(off / kInt4Tokens) * int4_record_bytes(D) +
+                        off % kInt4Tokens * (D / 2)
+                  : -1;
+      }
     }
-    return;
+    s_src[threadIdx.x] = src;
   }
-  const int column = t / p.page_size;
-  const int page = column < p.table_width ? p.table[int64_t(lo) * p.table_stride + column] : -1;
-  const bool known = page >= 0 && page < p.pool_pages;   // a page outside the pool reads as NaN
-  const int off = t % p.page_size, tok = off % kInt4Tokens;
-  for (int r = threadIdx.x / kLanes; r < 2 * p.heads_kv; r += kThreads / kLanes) {
-    const int part = r >= p.heads_kv ? 1 : 0;
-    const int h = r - part * p.heads_kv;
-    uint32_t codes = 0, params = 0x7e007e00u;
-    if (known) {
-      const unsigned char* rec =
-          p.pages + ((size_t(page) * p.heads_kv + h) * size_t(p.page_size / kInt4Tokens) + off / kInt4Tokens) *
-                        size_t(int4_record_bytes(D));
-      codes = *reinterpret_cast<const uint32_t*>(rec + (part * kInt4Tokens + tok) * (D / 2) + lane * 4);
-      params = *reinterpret_cast<const uint32_t*>(rec + kInt4Tokens * D + tok * 8 + part * 4);
-    }
-    const float s = __half2float(__ushort_as_half(uint16_t(params)));
-    const float m = __half2float(__ushort_as_half(uint16_t(params >> 16)));
-    float x[8];
+  __syncthreads();
+  const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+  const int items = 2 * p.heads_kv * kTokens;     // (K or V, head, token), tokens fastest
+  for (int i0 = group; i0 < items; i0 += kGroups * kAhead) {
+    uint2 codes[kAhead];
+    uint32_t params[kAhead];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = fmaf(s, float((codes >> (4 * e)) & 15u), m);
-    T* out = static_cast<T*>(part ? p.v_out : p.k_out) + (size_t(g) * p.heads_kv + h) * D + lane * 8;
-    *reinterpret_cast<uint4*>(out) =
-        make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
+    for (int a = 0; a < kAhead; ++a) {
+      const int item = i0 + a * kGroups;
+      codes[a] = make_uint2(0u, 0u);
+      params[a] = 0x7e007e00u;
+      if (item >= items) continue;
+      const int tok = item % kTokens, row = item / kTokens, h = row >> 1, part = row & 1;
+      const long long src = s_src[tok];
+      if (src >= 0) {
+        const unsigned char* at = p.pages + src + h * head_bytes;
+        const long long first = src % int4_record_bytes(D) / (D / 2);     // the token's row in its record
+        codes[a] = __ldg(reinterpret_cast<const uint2*>(at + part * (kInt4Tokens * D / 2) + lane * 8));
+        params[a] = __ldg(reinterpret_cast<const uint32_t*>(at + kInt4Tokens * D - first * (D / 2) + first * 8 + part * 4));
+      }
+    }
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) {
+      const int item = i0 + a * kGroups;
+      if (item >= items) continue;
+      const int tok = item % kTokens, row = item / kTokens, h = row >> 1, part = row & 1;
+      const long long src = s_src[tok];
+      if (src == -2) continue;
+      const size_t to = (size_t(g0 + tok) * p.heads_kv + h) * D + lane * 16;
+      uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(part ? p.v_out : p.k_out) + to);
+      if (src <= -3) {
+        const size_t from = (size_t(-3 - src) * p.heads_kv + h) * D + lane * 16;
+        const uint4* in = reinterpret_cast<const uint4*>(static_cast<const T*>(part ? p.v_new : p.k_new) + from);
+        out[0] = __ldg(in);
+        out[1] = __ldg(in + 1);
+        continue;
+      }
+      const float s = __half2float(__ushort_as_half(uint16_t(params[a])));
+      const float m = __half2float(__ushort_as_half(uint16_t(params[a] >> 16)));
+      const uint32_t c[2] = {codes[a].x, codes[a].y};
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = fmaf(s, float((c[i] >> (4 * e)) & 15u), m);
+        out[i] = make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
+      }
+    }
   }
 }
 
@@ -103,11 +144,11 @@ extern "C" int tb200_int4_cache_gather(const void* kv_pages, const int32_t* bloc
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool bf16 = dtype == TB200_BF16;
   if (dim == 64) {
-    if (bf16) int4_gather_kernel<__nv_bfloat16, 64><<<total_tokens, kThreads, 0, s>>>(p);
-    else int4_gather_kernel<__half, 64><<<total_tokens, kThreads, 0, s>>>(p);
+    if (bf16) int4_gather_kernel<__nv_bfloat16, 64><<<(total_tokens + kTokens - 1) / kTokens, kThreads, 0, s>>>(p);
+    else int4_gather_kernel<__half, 64><<<(total_tokens + kTokens - 1) / kTokens, kThreads, 0, s>>>(p);
   } else {
-    if (bf16) int4_gather_kernel<__nv_bfloat16, 128><<<total_tokens, kThreads, 0, s>>>(p);
-    else int4_gather_kernel<__half, 128><<<total_tokens, kThreads, 0, s>>>(p);
+    if (bf16) int4_gather_kernel<__nv_bfloat16, 128><<<(total_tokens + kTokens - 1) / kTokens, kThreads, 0, s>>>(p);
+    else int4_gather_kernel<__half, 128><<<(total_tokens + kTokens - 1) / kTokens, kThreads, 0, s>>>(p);
   }
   TB200_CUDA_CHECK(cudaGetLastError());
   return TB200_OK;

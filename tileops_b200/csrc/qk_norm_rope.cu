@@ -12,14 +12,15 @@
 // times a frequency has more digits than fp32 holds), reduced to a fraction of a turn, then one sincospif per (token,
 // frequency) shared by all heads through shared memory.  No table means no largest position and no gathers.
 //
-// HBM bound: every row is read and written once.
+// HBM bound: every row is read and written once.  A group of lanes holds a row, 8 values each, and requests kAhead rows
+// before it works on the first, while the block's angles are still being computed; where all dims rotate, a lane's values are
+// 4 of the first half and their 4 partners, so that the rotation needs no shuffles.
 #include "int4_cache.cuh"
 
 namespace tb200 {
 namespace {
 
 constexpr int kThreads = 128;
-constexpr int kMaxHalf = 128;      // rotary_dim / 2
 enum CacheKind { kNoCache = 0, kCache16 = 1, kCacheInt4 = 2 };
 
 struct RowsParams {
@@ -34,13 +35,28 @@ struct RowsParams {
   int heads, heads_kv, dim, rotary_dim, page_size;
   int rows;                          // rows of a token: q heads, k heads, then v heads when there is a cache
   int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head;   // strides in elements
-  int pool_tokens;
-  float eps;
+  int pool_tokens, tokens, block_tokens;
+  float eps, inv_dim;
 };
 
+// The 8 values of a lane: consecutive ones, or (kSplit) 4 at `at` and 4 at `at + half`.
+template <typename T, bool kSplit>
+__device__ __forceinline__ uint4 load_row(const T* p, int half) {
+  if constexpr (!kSplit) return __ldg(reinterpret_cast<const uint4*>(p));
+  const uint2 a = __ldg(reinterpret_cast<const uint2*>(p)), b = __ldg(reinterpret_cast<const uint2*>(p + half));
+  return make_uint4(a.x, a.y, b.x, b.y);
+}
+template <typename T, bool kSplit>
+__device__ __forceinline__ void store_row(T* p, int half, uint4 v) {
+  if constexpr (!kSplit) {
+    *reinterpret_cast<uint4*>(p) = v;
+  } else {
+    *reinterpret_cast<uint2*>(p) = make_uint2(v.x, v.y);
+    *reinterpret_cast<uint2*>(p + half) = make_uint2(v.z, v.w);
+  }
+}
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
-  const uint4 u = *reinterpret_cast<const uint4*>(p);
+__device__ __forceinline__ void unpack8(uint4 u, float (&x)[8]) {
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -53,127 +69,187 @@ template <typename T>
 __device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
   return make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
 }
+// Weights of a lane's values (element e at at + e, from e = 4 on at at2 + e - 4), kept in 16 bits where they come so.
 template <typename T>
-__device__ __forceinline__ void load_weight8(const void* w, int f32, int at, bool active, float (&x)[8]) {
+__device__ __forceinline__ void load_weight8(const void* w, int f32, int at, int at2, bool active, float (&x)[8]) {
+  if (!w || !active) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = 1.f;
-  if (!w || !active) return;
-  if (f32) {
+    for (int e = 0; e < 8; ++e) x[e] = 1.f;
+    return;
+  }
+  if (!f32 && (reinterpret_cast<uintptr_t>(w) & 7) == 0) {
+    const uint2 a = __ldg(reinterpret_cast<const uint2*>(static_cast<const T*>(w) + at));
+    const uint2 b = __ldg(reinterpret_cast<const uint2*>(static_cast<const T*>(w) + at2));
+    unpack8<T>(make_uint4(a.x, a.y, b.x, b.y), x);
+    return;
+  }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = static_cast<const float*>(w)[at + e];
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = float(static_cast<const T*>(w)[at + e]);
+  for (int e = 0; e < 8; ++e) {
+    const int d = e < 4 ? at + e : at2 + e - 4;
+    x[e] = f32 ? __ldg(static_cast<const float*>(w) + d) : float(static_cast<const T*>(w)[d]);
   }
 }
 
-// One block per token; kLanes lanes hold a row, 8 values each.
-template <typename T, int kLanes, int kCache, bool kNorm>
-__global__ void __launch_bounds__(kThreads) rows_kernel(RowsParams p) {
-  __shared__ float2 s_turn[kMaxHalf];
-  const int t = blockIdx.x;
-  const int lane = threadIdx.x & (kLanes - 1);
-  const int group = threadIdx.x / kLanes;
-  constexpr int kGroups = kThreads / kLanes;
-  const int at = lane * 8;
-  const bool active = at < p.dim;
-  const int half = p.rotary_dim >> 1;
-  float wq[8], wk[8];
-  if constexpr (kNorm) {
-    const double pos = double(p.positions[t]);
-    for (int j = threadIdx.x; j < half; j += kThreads) {
-      const double turns = pos * p.inv_turns[j];
-      float s, c;
-      sincospif(2.f * float(turns - rint(turns)), &s, &c);
-      s_turn[j] = make_float2(c, s);
-    }
-    load_weight8<T>(p.q_weight, p.weight_f32, at, active, wq);
-    load_weight8<T>(p.k_weight, p.weight_f32, at, active, wk);
-    __syncthreads();
-  }
-  const int slot = kCache != kNoCache ? p.slots[t] : -1;
-  const bool stored = slot >= 0 && slot < p.pool_tokens;
+constexpr int kMaxTokens = 8;      // of a block
 
-  for (int r0 = 0; r0 < p.rows; r0 += kGroups) {      // all lanes of a warp stay together for the shuffles
-    const int r = r0 + group;
-    const bool live = r < p.rows;
-    const bool is_q = r < p.heads, is_k = !is_q && r < p.heads + p.heads_kv;
-    const int h = is_q ? r : is_k ? r - p.heads : r - p.heads - p.heads_kv;
-    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (live && active) {
-      const T* src = is_q   ? static_cast<const T*>(p.q) + t * p.q_tok + h * p.q_head
-                     : is_k ? static_cast<const T*>(p.k) + t * p.k_tok + h * p.k_head
-                            : static_cast<const T*>(p.v) + t * p.v_tok + h * p.v_head;
-      load8(src + at, x);
+// A block of `block_tokens` tokens; kLanes lanes hold a row, 8 values each.
+template <typename T, int kLanes, int kCache, bool kNorm, bool kSplit, int kAhead>
+__global__ void __launch_bounds__(kThreads) rows_kernel(RowsParams p) {
+  constexpr int kGroups = kThreads / kLanes;
+  extern __shared__ float2 s_turn[];       // [block_tokens][half]: cos, sin
+  const int t0 = blockIdx.x * p.block_tokens;
+  const int lane = threadIdx.x & (kLanes - 1), group = threadIdx.x / kLanes;
+  const int half = p.rotary_dim >> 1;
+  const int at = kSplit ? lane * 4 : lane * 8, at2 = kSplit ? half + lane * 4 : at + 4;   // first and fifth value
+  const bool active = kSplit ? at < half : at < p.dim;
+  const int items = min(p.block_tokens, p.tokens - t0) * p.rows;
+  float wq[8], wk[8];
+  bool ready = !kNorm;
+
+  for (int i0 = group; i0 - group < items; i0 += kGroups * kAhead) {      // the lanes of a warp stay together
+    uint4 raw[kAhead];
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) {
+      const int item = i0 + a * kGroups;
+      raw[a] = make_uint4(0u, 0u, 0u, 0u);
+      if (item < items && active) {
+        const int tt = p.block_tokens == 1 ? 0 : item / p.rows, r = item - tt * p.rows;
+        const int64_t t = t0 + tt;
+        const T* src = r < p.heads                ? static_cast<const T*>(p.q) + t * p.q_tok + r * p.q_head
+                       : r < p.heads + p.heads_kv ? static_cast<const T*>(p.k) + t * p.k_tok + (r - p.heads) * p.k_head
+                                                  : static_cast<const T*>(p.v) + t * p.v_tok + (r - p.heads - p.heads_kv) * p.v_head;
+        raw[a] = load_row<T, kSplit>(src + at, half);
+      }
     }
     if constexpr (kNorm) {
-      float sum = 0.f;
+      if (!ready) {        // the angles, while the first rows are on their way
+        ready = true;
+        for (int j = threadIdx.x; j < p.block_tokens * half; j += kThreads) {
+          const int tt = j / half;
+          if (t0 + tt < p.tokens) {
+            const double turns = double(p.positions[t0 + tt]) * p.inv_turns[j - tt * half];
+            float s, c;
+            sincospif(2.f * float(turns - rint(turns)), &s, &c);
+            s_turn[j] = make_float2(c, s);
+          }
+        }
+        load_weight8<T>(p.q_weight, p.weight_f32, at, at2, active, wq);
+        load_weight8<T>(p.k_weight, p.weight_f32, at, at2, active, wk);
+        __syncthreads();
+      }
+    }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum = fmaf(x[e], x[e], sum);
+    for (int a = 0; a < kAhead; ++a) {
+      const int item = i0 + a * kGroups;
+      if (item - group >= items) break;          // the same for all lanes of the warp's groups
+      const int tt = p.block_tokens == 1 ? 0 : item / p.rows, r = item - tt * p.rows;
+      const int t = t0 + tt;
+      const bool live = item < items;
+      const bool is_q = r < p.heads, is_k = !is_q && r < p.heads + p.heads_kv;
+      const int h = is_q ? r : is_k ? r - p.heads : r - p.heads - p.heads_kv;
+      uint4 out = raw[a];
+      if constexpr (kNorm) {
+        float x[8];
+        unpack8<T>(raw[a], x);
+        float sum = 0.f;
 #pragma unroll
-      for (int o = 1; o < kLanes; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      const bool normed = is_q || is_k;
-      const float inv = rsqrtf(sum / float(p.dim) + p.eps);
-      float y[8];
+        for (int e = 0; e < 8; ++e) sum = fmaf(x[e], x[e], sum);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = normed ? x[e] * inv * (is_q ? wq[e] : wk[e]) : x[e];
-      const bool first = at < half, rotated = at < p.rotary_dim;
-      const int partner = rotated ? (first ? lane + half / 8 : lane - half / 8) : lane;
+        for (int o = 1; o < kLanes; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        const float inv = rsqrtf(fmaf(sum, p.inv_dim, p.eps));
+        float y[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float other = __shfl_sync(0xffffffffu, y[e], partner, kLanes);
-        x[e] = y[e];
-        if (rotated && normed) {
-          const float2 cs = s_turn[(first ? at : at - half) + e];
-          x[e] = first ? y[e] * cs.x - other * cs.y : y[e] * cs.x + other * cs.y;
+        for (int e = 0; e < 8; ++e) y[e] = x[e] * inv * (is_q ? wq[e] : wk[e]);
+        const float2* turn = s_turn + tt * half;
+        if constexpr (kSplit) {
+          const int j = active ? at : 0;      // lanes behind the row have no angles
+          const float4 cs0 = *reinterpret_cast<const float4*>(turn + j), cs1 = *reinterpret_cast<const float4*>(turn + j + 2);
+          const float c[4] = {cs0.x, cs0.z, cs1.x, cs1.z}, s[4] = {cs0.y, cs0.w, cs1.y, cs1.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            x[e] = y[e] * c[e] - y[e + 4] * s[e];
+            x[e + 4] = y[e + 4] * c[e] + y[e] * s[e];
+          }
+        } else {
+          const bool first = at < half, rotated = at < p.rotary_dim;
+          const int partner = rotated ? (first ? lane + half / 8 : lane - half / 8) : lane;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float other = __shfl_sync(0xffffffffu, y[e], partner, kLanes);
+            x[e] = y[e];
+            if (rotated) {
+              const float2 cs = turn[(first ? at : at - half) + e];
+              x[e] = first ? y[e] * cs.x - other * cs.y : y[e] * cs.x + other * cs.y;
+            }
+          }
+        }
+        if (is_q || is_k) out = pack8<T>(x);       // v rows pass as they are
+      }
+      if (live && active) {
+        if (is_q)
+          store_row<T, kSplit>(static_cast<T*>(p.q_out) + (size_t(t) * p.heads + h) * p.dim + at, half, out);
+        else if (is_k && p.k_out)
+          store_row<T, kSplit>(static_cast<T*>(p.k_out) + (size_t(t) * p.heads_kv + h) * p.dim + at, half, out);
+      }
+      if constexpr (kCache != kNoCache) {
+        const int slot = live && !is_q ? __ldg(p.slots + t) : -1;
+        const bool stored = slot >= 0 && slot < p.pool_tokens;
+        if constexpr (kCache == kCache16) {
+          if (stored && active)
+            store_row<T, kSplit>(static_cast<T*>(is_k ? p.k_cache : p.v_cache) + (size_t(slot) * p.heads_kv + h) * p.dim + at,
+                                 half, out);
+        } else {
+          if (!__any_sync(0xffffffffu, stored)) continue;
+          float z[8];
+          unpack8<T>(out, z);
+          uint32_t params;
+          const uint32_t codes = int4_quantise<kLanes>(z, slot & 1, params);
+          if (stored) {
+            unsigned char* rec = static_cast<unsigned char*>(p.k_cache) +
+                                 int4_record_of(slot, h, p.heads_kv, p.page_size, p.dim);
+            const int tok = slot % kInt4Tokens, part = is_k ? 0 : 1;
+            unsigned char* row = rec + (part * kInt4Tokens + tok) * (p.dim / 2);
+            if constexpr (kSplit) {
+              *reinterpret_cast<uint16_t*>(row + lane * 2) = uint16_t(codes);
+              *reinterpret_cast<uint16_t*>(row + p.dim / 4 + lane * 2) = uint16_t(codes >> 16);
+            } else {
+              *reinterpret_cast<uint32_t*>(row + lane * 4) = codes;
+            }
+            if (lane == 0) *reinterpret_cast<uint32_t*>(rec + kInt4Tokens * p.dim + tok * 8 + part * 4) = params;
+          }
         }
       }
     }
-    const uint4 out = pack8<T>(x);
-    if (live && active) {
-      if (is_q) {
-        if (p.q_out) *reinterpret_cast<uint4*>(static_cast<T*>(p.q_out) + (size_t(t) * p.heads + h) * p.dim + at) = out;
-      } else if (is_k && p.k_out) {
-        *reinterpret_cast<uint4*>(static_cast<T*>(p.k_out) + (size_t(t) * p.heads_kv + h) * p.dim + at) = out;
-      }
-    }
-    if constexpr (kCache == kCache16) {
-      if (live && active && !is_q && stored) {
-        T* pool = static_cast<T*>(is_k ? p.k_cache : p.v_cache);
-        *reinterpret_cast<uint4*>(pool + (size_t(slot) * p.heads_kv + h) * p.dim + at) = out;
-      }
-    }
-    if constexpr (kCache == kCacheInt4) {
-      float z[8];
-      const uint32_t w[4] = {out.x, out.y, out.z, out.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 f = unpack2<T>(w[i]);
-        z[2 * i] = f.x;
-        z[2 * i + 1] = f.y;
-      }
-      uint32_t params;
-      const uint32_t codes = int4_quantise<kLanes>(z, slot & 1, params);
-      if (live && !is_q && stored) {
-        unsigned char* rec = static_cast<unsigned char*>(p.k_cache) +
-                             int4_record_of(slot, h, p.heads_kv, p.page_size, p.dim);
-        const int tok = slot % kInt4Tokens;
-        const int part = is_k ? 0 : 1;
-        *reinterpret_cast<uint32_t*>(rec + (part * kInt4Tokens + tok) * (p.dim / 2) + lane * 4) = codes;
-        if (lane == 0) *reinterpret_cast<uint32_t*>(rec + kInt4Tokens * p.dim + tok * 8 + part * 4) = params;
-      }
-    }
   }
 }
 
+template <typename T, int kLanes, int kCache, bool kNorm>
+void launch_lanes(RowsParams p, int tokens, cudaStream_t s) {
+  constexpr int kGroups = kThreads / kLanes;
+  p.tokens = tokens;
+  p.inv_dim = 1.f / float(p.dim);
+  // about kRowsPerGroup rows for every group of lanes, however few heads there are
+  constexpr int kRowsPerGroup = 6;
+  p.block_tokens = kRowsPerGroup * kGroups / p.rows;
+  if (p.block_tokens < 1) p.block_tokens = 1;
+  if (p.block_tokens > kMaxTokens) p.block_tokens = kMaxTokens;
+  // few tokens: one to a block, so that they spread over the SMs
+  if (tokens < sm_count() * 4) p.block_tokens = 1;
+  const int blocks = (tokens + p.block_tokens - 1) / p.block_tokens;
+  const size_t smem = kNorm ? size_t(p.block_tokens) * (p.rotary_dim / 2) * sizeof(float2) : 0;
+  if (kNorm && p.rotary_dim == p.dim && p.dim % 16 == 0)
+    rows_kernel<T, kLanes, kCache, kNorm, kNorm, kRowsPerGroup><<<blocks, kThreads, smem, s>>>(p);
+  else
+    rows_kernel<T, kLanes, kCache, kNorm, false, kRowsPerGroup><<<blocks, kThreads, smem, s>>>(p);
+}
 template <typename T, int kCache, bool kNorm>
 void launch_rows(const RowsParams& p, int tokens, cudaStream_t s) {
   if (p.dim <= 64)
-    rows_kernel<T, 8, kCache, kNorm><<<tokens, kThreads, 0, s>>>(p);
+    launch_lanes<T, 8, kCache, kNorm>(p, tokens, s);
   else if (p.dim <= 128)
-    rows_kernel<T, 16, kCache, kNorm><<<tokens, kThreads, 0, s>>>(p);
+    launch_lanes<T, 16, kCache, kNorm>(p, tokens, s);
   else if constexpr (kCache != kCacheInt4)
-    rows_kernel<T, 32, kCache, kNorm><<<tokens, kThreads, 0, s>>>(p);
+    launch_lanes<T, 32, kCache, kNorm>(p, tokens, s);
 }
 
 // 16-byte rows: the base and both strides
