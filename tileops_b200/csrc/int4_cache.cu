@@ -96,14 +96,22 @@ __global__ void __launch_bounds__(kThreads) int4_gather_kernel(GatherParams p) {
         out[1] = __ldg(in + 1);
         continue;
       }
-      const float s = __half2float(__ushort_as_half(uint16_t(params[a])));
-      const float m = __half2float(__ushort_as_half(uint16_t(params[a] >> 16)));
+      // a nibble masked into the low bits of a float16 is the number c * 2^-24: two codes per mask, no conversion
+      const float2 sm = f16x2_to_f32x2(params[a]);
+      const float lo = sm.x * 16777216.f, hi = sm.x * 1048576.f, m = sm.y;
       const uint32_t c[2] = {codes[a].x, codes[a].y};
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         float x[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = fmaf(s, float((c[i] >> (4 * e)) & 15u), m);
+        for (int b = 0; b < 2; ++b) {
+          const uint32_t v = b ? c[i] >> 8 : c[i];
+          const float2 even = f16x2_to_f32x2(v & 0x000f000fu), odd = f16x2_to_f32x2(v & 0x00f000f0u);
+          x[2 * b] = fmaf(lo, even.x, m);
+          x[2 * b + 1] = fmaf(hi, odd.x, m);
+          x[2 * b + 4] = fmaf(lo, even.y, m);
+          x[2 * b + 5] = fmaf(hi, odd.y, m);
+        }
         out[i] = make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
       }
     }

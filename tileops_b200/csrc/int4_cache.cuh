@@ -36,42 +36,49 @@ __device__ __forceinline__ size_t int4_record_of(int slot, int head, int heads_k
          size_t(int4_record_bytes(dim));
 }
 
-// Quantises 8 consecutive values of a row that kLanes neighbouring lanes hold together (8 values per lane, all lanes of
-// the group active).  Returns the 8 codes as 4 bytes; `params` (scale in the low half, offset in the high half) is the
-// same on every lane of the group.
+// min and max that pass a NaN on
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float y;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+
+// Quantises 8 values of a row that kLanes neighbouring lanes hold together (8 values per lane, all lanes of the group
+// active).  Returns the 8 codes as 4 bytes; `params` (scale in the low half, offset in the high half) is the same on every
+// lane of the group.  Values beyond the clamp need no clamp of their own: their code lies beyond 0 or 15 and is clamped.
+// A code becomes an integer by adding 1.5 * 2^23 (round to nearest even, as rint), and the eight are put together by
+// multiply-adds modulo 2^32, from which the constants' sum is taken off: the conversion and shift units stay free.
 template <int kLanes>
-__device__ __forceinline__ uint32_t int4_quantise(const float (&v)[8], bool odd_slot, uint32_t& params) {
-  float x[8];
-  float lo = kInt4Clamp, hi = -kInt4Clamp;
-  bool bad = false;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    bad |= v[e] != v[e];
-    x[e] = fminf(fmaxf(v[e], -kInt4Clamp), kInt4Clamp);
-    lo = fminf(lo, x[e]);
-    hi = fmaxf(hi, x[e]);
-  }
+__device__ __forceinline__ uint32_t int4_quantise(const float (&x)[8], bool odd_slot, uint32_t& params) {
+  float lo = min_nan(min_nan(min_nan(x[0], x[1]), min_nan(x[2], x[3])), min_nan(min_nan(x[4], x[5]), min_nan(x[6], x[7])));
+  float hi = max_nan(max_nan(max_nan(x[0], x[1]), max_nan(x[2], x[3])), max_nan(max_nan(x[4], x[5]), max_nan(x[6], x[7])));
 #pragma unroll
   for (int o = 1; o < kLanes; o <<= 1) {
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
   }
-  const unsigned votes = __ballot_sync(0xffffffffu, bad);
-  const unsigned group = (kLanes == 32 ? 0xffffffffu : ((1u << kLanes) - 1u) << (threadIdx.x & 31 & ~(kLanes - 1)));
+  lo = min_nan(max_nan(lo, -kInt4Clamp), kInt4Clamp);
+  hi = min_nan(max_nan(hi, -kInt4Clamp), kInt4Clamp);
   const __half step = __float2half_rn(__fdiv_rn(hi - lo, 15.f));
   const __half scale = odd_slot ? __hneg(step) : step;
   const __half offset = __float2half_rn(odd_slot ? hi : lo);
   const float s = __half2float(scale), m = __half2float(offset);
   const float inverse = s == 0.f ? 0.f : __frcp_rn(s);
+  constexpr float kMagic = 12582912.f;
+  constexpr uint32_t kMagicBits = 0x4b400000u;
   uint32_t codes = 0;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float c = fminf(fmaxf(rintf(__fmul_rn(x[e] - m, inverse)), 0.f), 15.f);
-    codes |= uint32_t(c) << (4 * e);
+  for (int e = 7; e >= 0; --e) {
+    const float c = fminf(fmaxf(__fmul_rn(x[e] - m, inverse), 0.f), 15.f);   // a NaN becomes 0
+    codes = codes * 16u + __float_as_uint(__fadd_rn(c, kMagic));
   }
   params = uint32_t(__half_as_ushort(scale)) | (uint32_t(__half_as_ushort(offset)) << 16);
-  if (votes & group) { params = 0x7e007e00u; codes = 0; }
-  return codes;
+  return codes - kMagicBits * 0x11111111u;
 }
 
 }  // namespace tb200

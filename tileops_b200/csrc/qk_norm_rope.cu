@@ -12,9 +12,11 @@
 // times a frequency has more digits than fp32 holds), reduced to a fraction of a turn, then one sincospif per (token,
 // frequency) shared by all heads through shared memory.  No table means no largest position and no gathers.
 //
-// HBM bound: every row is read and written once.  A group of lanes holds a row, 8 values each, and requests kAhead rows
+// HBM bound: every row is read and written once.  A group of lanes holds a row, 8 values each, and requests four rows
 // before it works on the first, while the block's angles are still being computed; where all dims rotate, a lane's values are
 // 4 of the first half and their 4 partners, so that the rotation needs no shuffles.
+#include <type_traits>
+
 #include "int4_cache.cuh"
 
 namespace tb200 {
@@ -91,136 +93,144 @@ __device__ __forceinline__ void load_weight8(const void* w, int f32, int at, int
 }
 
 constexpr int kMaxTokens = 8;      // of a block
+enum RowKind { kRowQ = 0, kRowK = 1, kRowV = 2 };
 
-// A block of `block_tokens` tokens; kLanes lanes hold a row, 8 values each.
-template <typename T, int kLanes, int kCache, bool kNorm, bool kSplit, int kAhead>
+// A block of `block_tokens` tokens; kLanes lanes hold a row, 8 values each.  q, k and v rows are walked one kind after the
+// other, so that weights, pointers and what becomes of a row are settled outside the loop over rows.
+template <typename T, int kLanes, int kCache, bool kNorm, bool kSplit>
 __global__ void __launch_bounds__(kThreads) rows_kernel(RowsParams p) {
   constexpr int kGroups = kThreads / kLanes;
   extern __shared__ float2 s_turn[];       // [block_tokens][half]: cos, sin
   const int t0 = blockIdx.x * p.block_tokens;
+  const int n_tokens = min(p.block_tokens, p.tokens - t0);
   const int lane = threadIdx.x & (kLanes - 1), group = threadIdx.x / kLanes;
   const int half = p.rotary_dim >> 1;
   const int at = kSplit ? lane * 4 : lane * 8, at2 = kSplit ? half + lane * 4 : at + 4;   // first and fifth value
   const bool active = kSplit ? at < half : at < p.dim;
-  const int items = min(p.block_tokens, p.tokens - t0) * p.rows;
-  float wq[8], wk[8];
   bool ready = !kNorm;
 
-  for (int i0 = group; i0 - group < items; i0 += kGroups * kAhead) {      // the lanes of a warp stay together
-    uint4 raw[kAhead];
+  // kAhead rows of one kind, from item i0 (token of the block * rows + row) in steps of kGroups
+  auto walk = [&](auto kind_, auto ahead_, const T* src, int64_t tok_stride, int64_t head_stride, int rows, const void* weight) {
+    constexpr int kKind = decltype(kind_)::value, kAhead = decltype(ahead_)::value;
+    constexpr bool kNormed = kNorm && kKind != kRowV;
+    const int items = n_tokens * rows;
+    src += t0 * tok_stride + at;
+    float w[8];
+    for (int i0 = group; i0 - group < items; i0 += kGroups * kAhead) {      // the lanes of a warp stay together
+      uint4 raw[kAhead];
 #pragma unroll
-    for (int a = 0; a < kAhead; ++a) {
-      const int item = i0 + a * kGroups;
-      raw[a] = make_uint4(0u, 0u, 0u, 0u);
-      if (item < items && active) {
-        const int tt = p.block_tokens == 1 ? 0 : item / p.rows, r = item - tt * p.rows;
-        const int64_t t = t0 + tt;
-        const T* src = r < p.heads                ? static_cast<const T*>(p.q) + t * p.q_tok + r * p.q_head
-                       : r < p.heads + p.heads_kv ? static_cast<const T*>(p.k) + t * p.k_tok + (r - p.heads) * p.k_head
-                                                  : static_cast<const T*>(p.v) + t * p.v_tok + (r - p.heads - p.heads_kv) * p.v_head;
-        raw[a] = load_row<T, kSplit>(src + at, half);
+      for (int a = 0; a < kAhead; ++a) {
+        const int item = i0 + a * kGroups;
+        const int tt = n_tokens == 1 ? 0 : item / rows, r = item - tt * rows;
+        raw[a] = item < items && active ? load_row<T, kSplit>(src + tt * tok_stride + r * head_stride, half)
+                                        : make_uint4(0u, 0u, 0u, 0u);
       }
-    }
-    if constexpr (kNorm) {
-      if (!ready) {        // the angles, while the first rows are on their way
-        ready = true;
-        for (int j = threadIdx.x; j < p.block_tokens * half; j += kThreads) {
-          const int tt = j / half;
-          if (t0 + tt < p.tokens) {
+      if constexpr (kNormed) {
+        if (i0 == group) load_weight8<T>(weight, p.weight_f32, at, at2, active, w);
+        if (!ready) {        // the angles, while the first rows are on their way
+          ready = true;
+          for (int j = threadIdx.x; j < n_tokens * half; j += kThreads) {
+            const int tt = n_tokens == 1 ? 0 : j / half;
             const double turns = double(p.positions[t0 + tt]) * p.inv_turns[j - tt * half];
             float s, c;
             sincospif(2.f * float(turns - rint(turns)), &s, &c);
             s_turn[j] = make_float2(c, s);
           }
+          __syncthreads();
         }
-        load_weight8<T>(p.q_weight, p.weight_f32, at, at2, active, wq);
-        load_weight8<T>(p.k_weight, p.weight_f32, at, at2, active, wk);
-        __syncthreads();
       }
-    }
 #pragma unroll
-    for (int a = 0; a < kAhead; ++a) {
-      const int item = i0 + a * kGroups;
-      if (item - group >= items) break;          // the same for all lanes of the warp's groups
-      const int tt = p.block_tokens == 1 ? 0 : item / p.rows, r = item - tt * p.rows;
-      const int t = t0 + tt;
-      const bool live = item < items;
-      const bool is_q = r < p.heads, is_k = !is_q && r < p.heads + p.heads_kv;
-      const int h = is_q ? r : is_k ? r - p.heads : r - p.heads - p.heads_kv;
-      uint4 out = raw[a];
-      if constexpr (kNorm) {
-        float x[8];
-        unpack8<T>(raw[a], x);
-        float sum = 0.f;
+      for (int a = 0; a < kAhead; ++a) {
+        const int item = i0 + a * kGroups;
+        if (item - group >= items) break;          // the same for the whole block
+        const int tt = n_tokens == 1 ? 0 : item / rows, r = item - tt * rows;
+        const bool live = item < items;
+        uint4 out = raw[a];
+        if constexpr (kNormed) {
+          float x[8];
+          unpack8<T>(raw[a], x);
+          float sum = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sum = fmaf(x[e], x[e], sum);
+          for (int e = 0; e < 8; ++e) sum = fmaf(x[e], x[e], sum);
 #pragma unroll
-        for (int o = 1; o < kLanes; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        const float inv = rsqrtf(fmaf(sum, p.inv_dim, p.eps));
-        float y[8];
+          for (int o = 1; o < kLanes; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+          const float inv = rsqrtf(fmaf(sum, p.inv_dim, p.eps));
+          float y[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = x[e] * inv * (is_q ? wq[e] : wk[e]);
-        const float2* turn = s_turn + tt * half;
-        if constexpr (kSplit) {
-          const int j = active ? at : 0;      // lanes behind the row have no angles
-          const float4 cs0 = *reinterpret_cast<const float4*>(turn + j), cs1 = *reinterpret_cast<const float4*>(turn + j + 2);
-          const float c[4] = {cs0.x, cs0.z, cs1.x, cs1.z}, s[4] = {cs0.y, cs0.w, cs1.y, cs1.w};
+          for (int e = 0; e < 8; ++e) y[e] = x[e] * inv * w[e];
+          const float2* turn = s_turn + tt * half;
+          if constexpr (kSplit) {
+            const int j = active ? at : 0;      // lanes behind the row have no angles
+            const float4 cs0 = *reinterpret_cast<const float4*>(turn + j), cs1 = *reinterpret_cast<const float4*>(turn + j + 2);
+            const float c[4] = {cs0.x, cs0.z, cs1.x, cs1.z}, s[4] = {cs0.y, cs0.w, cs1.y, cs1.w};
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            x[e] = y[e] * c[e] - y[e + 4] * s[e];
-            x[e + 4] = y[e + 4] * c[e] + y[e] * s[e];
-          }
-        } else {
-          const bool first = at < half, rotated = at < p.rotary_dim;
-          const int partner = rotated ? (first ? lane + half / 8 : lane - half / 8) : lane;
+            for (int e = 0; e < 4; ++e) {
+              x[e] = y[e] * c[e] - y[e + 4] * s[e];
+              x[e + 4] = y[e + 4] * c[e] + y[e] * s[e];
+            }
+          } else {
+            const bool first = at < half, rotated = at < p.rotary_dim;
+            const int partner = rotated ? (first ? lane + half / 8 : lane - half / 8) : lane;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float other = __shfl_sync(0xffffffffu, y[e], partner, kLanes);
-            x[e] = y[e];
-            if (rotated) {
-              const float2 cs = turn[(first ? at : at - half) + e];
-              x[e] = first ? y[e] * cs.x - other * cs.y : y[e] * cs.x + other * cs.y;
+            for (int e = 0; e < 8; ++e) {
+              const float other = __shfl_sync(0xffffffffu, y[e], partner, kLanes);
+              x[e] = y[e];
+              if (rotated) {
+                const float2 cs = turn[(first ? at : at - half) + e];
+                x[e] = first ? y[e] * cs.x - other * cs.y : y[e] * cs.x + other * cs.y;
+              }
             }
           }
+          out = pack8<T>(x);
         }
-        if (is_q || is_k) out = pack8<T>(x);       // v rows pass as they are
-      }
-      if (live && active) {
-        if (is_q)
-          store_row<T, kSplit>(static_cast<T*>(p.q_out) + (size_t(t) * p.heads + h) * p.dim + at, half, out);
-        else if (is_k && p.k_out)
-          store_row<T, kSplit>(static_cast<T*>(p.k_out) + (size_t(t) * p.heads_kv + h) * p.dim + at, half, out);
-      }
-      if constexpr (kCache != kNoCache) {
-        const int slot = live && !is_q ? __ldg(p.slots + t) : -1;
-        const bool stored = slot >= 0 && slot < p.pool_tokens;
-        if constexpr (kCache == kCache16) {
-          if (stored && active)
-            store_row<T, kSplit>(static_cast<T*>(is_k ? p.k_cache : p.v_cache) + (size_t(slot) * p.heads_kv + h) * p.dim + at,
-                                 half, out);
+        const int t = t0 + tt;
+        if constexpr (kKind == kRowQ) {
+          if (live && active)
+            store_row<T, kSplit>(static_cast<T*>(p.q_out) + (size_t(t) * p.heads + r) * p.dim + at, half, out);
         } else {
-          if (!__any_sync(0xffffffffu, stored)) continue;
-          float z[8];
-          unpack8<T>(out, z);
-          uint32_t params;
-          const uint32_t codes = int4_quantise<kLanes>(z, slot & 1, params);
-          if (stored) {
-            unsigned char* rec = static_cast<unsigned char*>(p.k_cache) +
-                                 int4_record_of(slot, h, p.heads_kv, p.page_size, p.dim);
-            const int tok = slot % kInt4Tokens, part = is_k ? 0 : 1;
-            unsigned char* row = rec + (part * kInt4Tokens + tok) * (p.dim / 2);
-            if constexpr (kSplit) {
-              *reinterpret_cast<uint16_t*>(row + lane * 2) = uint16_t(codes);
-              *reinterpret_cast<uint16_t*>(row + p.dim / 4 + lane * 2) = uint16_t(codes >> 16);
+          if (kKind == kRowK && p.k_out && live && active)
+            store_row<T, kSplit>(static_cast<T*>(p.k_out) + (size_t(t) * p.heads_kv + r) * p.dim + at, half, out);
+          if constexpr (kCache != kNoCache) {
+            const int slot = live ? __ldg(p.slots + t) : -1;
+            const bool stored = slot >= 0 && slot < p.pool_tokens;
+            if constexpr (kCache == kCache16) {
+              if (stored && active)
+                store_row<T, kSplit>(static_cast<T*>(kKind == kRowK ? p.k_cache : p.v_cache) +
+                                         (size_t(slot) * p.heads_kv + r) * p.dim + at, half, out);
             } else {
-              *reinterpret_cast<uint32_t*>(row + lane * 4) = codes;
+              float z[8];
+              unpack8<T>(out, z);
+              uint32_t params;
+              const uint32_t codes = int4_quantise<kLanes>(z, slot & 1, params);
+              if (stored) {
+                unsigned char* rec = static_cast<unsigned char*>(p.k_cache) +
+                                     int4_record_of(slot, r, p.heads_kv, p.page_size, p.dim);
+                constexpr int part = kKind == kRowK ? 0 : 1;
+                const int tok = slot % kInt4Tokens;
+                unsigned char* row = rec + (part * kInt4Tokens + tok) * (p.dim / 2);
+                if constexpr (kSplit) {
+                  *reinterpret_cast<uint16_t*>(row + lane * 2) = uint16_t(codes);
+                  *reinterpret_cast<uint16_t*>(row + p.dim / 4 + lane * 2) = uint16_t(codes >> 16);
+                } else {
+                  *reinterpret_cast<uint32_t*>(row + lane * 4) = codes;
+                }
+                if (lane == 0) *reinterpret_cast<uint32_t*>(rec + kInt4Tokens * p.dim + tok * 8 + part * 4) = params;
+              }
             }
-            if (lane == 0) *reinterpret_cast<uint32_t*>(rec + kInt4Tokens * p.dim + tok * 8 + part * 4) = params;
           }
         }
       }
     }
-  }
+  };
+  using Q = std::integral_constant<int, kRowQ>;
+  using K = std::integral_constant<int, kRowK>;
+  using V = std::integral_constant<int, kRowV>;
+  using Ahead = std::integral_constant<int, 4>;
+  if constexpr (kNorm)
+    walk(Q{}, Ahead{}, static_cast<const T*>(p.q), p.q_tok, p.q_head, p.heads, p.q_weight);
+  walk(K{}, Ahead{}, static_cast<const T*>(p.k), p.k_tok, p.k_head, p.heads_kv, p.k_weight);
+  if constexpr (kCache != kNoCache)
+    walk(V{}, Ahead{}, static_cast<const T*>(p.v), p.v_tok, p.v_head, p.heads_kv, nullptr);
 }
 
 template <typename T, int kLanes, int kCache, bool kNorm>
@@ -238,9 +248,9 @@ void launch_lanes(RowsParams p, int tokens, cudaStream_t s) {
   const int blocks = (tokens + p.block_tokens - 1) / p.block_tokens;
   const size_t smem = kNorm ? size_t(p.block_tokens) * (p.rotary_dim / 2) * sizeof(float2) : 0;
   if (kNorm && p.rotary_dim == p.dim && p.dim % 16 == 0)
-    rows_kernel<T, kLanes, kCache, kNorm, kNorm, kRowsPerGroup><<<blocks, kThreads, smem, s>>>(p);
+    rows_kernel<T, kLanes, kCache, kNorm, kNorm><<<blocks, kThreads, smem, s>>>(p);
   else
-    rows_kernel<T, kLanes, kCache, kNorm, false, kRowsPerGroup><<<blocks, kThreads, smem, s>>>(p);
+    rows_kernel<T, kLanes, kCache, kNorm, false><<<blocks, kThreads, smem, s>>>(p);
 }
 template <typename T, int kCache, bool kNorm>
 void launch_rows(const RowsParams& p, int tokens, cudaStream_t s) {
