@@ -189,6 +189,38 @@ def test_norm_rope_matches_64_bits(T, H, Hkv, D, rotary, dtype):
         assert_within(got, ref, norm_tolerance(ref, dtype), f"{T} {H} {Hkv} {D} {rotary}")
 
 
+@pytest.mark.parametrize("T", [600, 1021, 2500])
+@pytest.mark.parametrize("H,Hkv,D,rotary", [(1, 1, 64, 64), (7, 1, 128, 128), (20, 5, 80, 32), (3, 3, 96, 96), (2, 1, 256, 64),
+                                            (32, 8, 128, 128), (5, 2, 8, 0)])
+def test_many_tokens_share_blocks(T, H, Hkv, D, rotary):
+    """Batches large enough for blocks of several tokens: the whole call equals calls on pieces of it (one token a block),
+    which the tests above hold to 64 bits; nothing but the rows is written."""
+    dtype = torch.bfloat16
+    q, k, v, qw, kw = qkv(T, H, Hkv, D, dtype, T, fused=True)
+    pos = torch.randint(0, 9999, (T,), dtype=torch.int32, device=DEV)
+    pool = T + 5
+    slots = torch.randperm(pool, device=DEV)[:T].to(torch.int32)
+    slots[T // 3] = -1
+    op = ops.QKNormRopeKVCacheAppendFwdOp(H, Hkv, D, rotary)
+    pages = [torch.zeros(pool, Hkv, D, dtype=dtype, device=DEV) for _ in range(4)]
+    q1, k1 = op(q, k, v, qw, kw, pos, slots, pages[0], pages[1], return_k=True)
+    for i in range(0, T, 200):
+        j = slice(i, i + 200)
+        q2, k2 = op(q[j], k[j], v[j], qw, kw, pos[j], slots[j], pages[2], pages[3], return_k=True)
+        assert torch.equal(q1[j], q2) and torch.equal(k1[j], k2)
+    assert torch.equal(pages[0], pages[2]) and torch.equal(pages[1], pages[3])
+    if D in (64, 128):
+        page = 16
+        four = [torch.zeros(-(-pool // page), Hkv, F.int4_page_bytes(page, D), dtype=torch.uint8, device=DEV) for _ in range(3)]
+        op4, append = ops.QKNormRopeInt4KVCacheAppendFwdOp(H, Hkv, D, page, rotary), ops.Int4KVCacheAppendFwdOp(Hkv, D, page)
+        assert torch.equal(op4(q, k, v, qw, kw, pos, slots, four[0]), q1)
+        append(k1, v, slots, four[1])
+        for i in range(0, T, 200):
+            j = slice(i, i + 200)
+            append(k1[j], v[j], slots[j], four[2])
+        assert torch.equal(four[0], four[1]) and torch.equal(four[1], four[2])
+
+
 def test_norm_rope_reads_parts_of_one_projection_and_odd_strides():
     T, H, Hkv, D = 9, 6, 2, 128
     q, k, v, qw, kw = qkv(T, H, Hkv, D, torch.bfloat16, 5, fused=True)

@@ -71,11 +71,19 @@ __device__ __forceinline__ uint32_t int4_quantise(const float (&x)[8], bool odd_
   const float inverse = s == 0.f ? 0.f : __frcp_rn(s);
   constexpr float kMagic = 12582912.f;
   constexpr uint32_t kMagicBits = 0x4b400000u;
+  // Codes stay between 0 and 15 by themselves unless the scale is a subnormal, an end was rounded or clamped, or the row has
+  // a NaN: the scale's rounding moves 15 steps by 15 x 2^-11 of one.
+  const bool plain = fabsf(s) >= 6.103515625e-5f && m == (odd_slot ? hi : lo) && lo > -kInt4Clamp && hi < kInt4Clamp;
   uint32_t codes = 0;
+  if (__all_sync(0xffffffffu, plain)) {
 #pragma unroll
-  for (int e = 7; e >= 0; --e) {
-    const float c = fminf(fmaxf(__fmul_rn(x[e] - m, inverse), 0.f), 15.f);   // a NaN becomes 0
-    codes = codes * 16u + __float_as_uint(__fadd_rn(c, kMagic));
+    for (int e = 7; e >= 0; --e) codes = codes * 16u + __float_as_uint(__fadd_rn(__fmul_rn(x[e] - m, inverse), kMagic));
+  } else {
+#pragma unroll
+    for (int e = 7; e >= 0; --e) {
+      const float c = fminf(fmaxf(__fmul_rn(x[e] - m, inverse), 0.f), 15.f);   // a NaN becomes 0
+      codes = codes * 16u + __float_as_uint(__fadd_rn(c, kMagic));
+    }
   }
   params = uint32_t(__half_as_ushort(scale)) | (uint32_t(__half_as_ushort(offset)) << 16);
   return codes - kMagicBits * 0x11111111u;

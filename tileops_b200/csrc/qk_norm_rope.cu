@@ -36,7 +36,8 @@ struct RowsParams {
   void *k_cache, *v_cache;           // kCacheInt4: k_cache is the one pool
   int heads, heads_kv, dim, rotary_dim, page_size;
   int rows;                          // rows of a token: q heads, k heads, then v heads when there is a cache
-  int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head;   // strides in elements
+  int q_tok, q_head, k_tok, k_head, v_tok, v_head;       // strides in elements
+  unsigned by_heads, by_heads_kv, by_half;               // reciprocals for the divisions by heads, heads_kv and rotary_dim / 2
   int pool_tokens, tokens, block_tokens;
   float eps, inv_dim;
 };
@@ -93,6 +94,10 @@ __device__ __forceinline__ void load_weight8(const void* w, int f32, int at, int
 }
 
 constexpr int kMaxTokens = 8;      // of a block
+
+// n / d for n < 2^16 by the reciprocal 2^32 / d, rounded up (0 where d is 1)
+inline unsigned reciprocal(int d) { return d <= 1 ? 0u : 0xffffffffu / unsigned(d) + 1u; }
+__device__ __forceinline__ int divide(int n, unsigned by) { return by ? int(__umulhi(unsigned(n), by)) : n; }
 enum RowKind { kRowQ = 0, kRowK = 1, kRowV = 2 };
 
 // A block of `block_tokens` tokens; kLanes lanes hold a row, 8 values each.  q, k and v rows are walked one kind after the
@@ -101,50 +106,80 @@ template <typename T, int kLanes, int kCache, bool kNorm, bool kSplit>
 __global__ void __launch_bounds__(kThreads) rows_kernel(RowsParams p) {
   constexpr int kGroups = kThreads / kLanes;
   extern __shared__ float2 s_turn[];       // [block_tokens][half]: cos, sin
+  // where the tokens' rows go: element (16-bit cache) or byte of the record (4-bit) of head 0, -1: nowhere; row of the record
+  __shared__ long long s_to[kMaxTokens];
+  __shared__ int s_row[kMaxTokens];
   const int t0 = blockIdx.x * p.block_tokens;
   const int n_tokens = min(p.block_tokens, p.tokens - t0);
   const int lane = threadIdx.x & (kLanes - 1), group = threadIdx.x / kLanes;
   const int half = p.rotary_dim >> 1;
   const int at = kSplit ? lane * 4 : lane * 8, at2 = kSplit ? half + lane * 4 : at + 4;   // first and fifth value
   const bool active = kSplit ? at < half : at < p.dim;
-  bool ready = !kNorm;
+  const long long head_bytes = (long long)(p.page_size / kInt4Tokens) * int4_record_bytes(p.dim);
+  bool ready = false;
+
+  // angles and destinations of the block's tokens, worked out while the first rows are on their way
+  auto prepare = [&] {
+    if (kCache != kNoCache && threadIdx.x < n_tokens) {
+      const int slot = p.slots[t0 + threadIdx.x];
+      long long to = -1;
+      if (slot >= 0 && slot < p.pool_tokens) {
+        if constexpr (kCache == kCacheInt4) {
+          const int page = slot / p.page_size, off = slot - page * p.page_size;
+          to = (long long)page * p.heads_kv * head_bytes + (long long)(off / kInt4Tokens) * int4_record_bytes(p.dim);
+          s_row[threadIdx.x] = off % kInt4Tokens;      // a record begins at an even slot: the parity is the slot's
+        } else {
+          to = (long long)slot * p.heads_kv * p.dim;
+        }
+      }
+      s_to[threadIdx.x] = to;
+    }
+    if constexpr (kNorm) {
+      for (int j = threadIdx.x; j < n_tokens * half; j += kThreads) {
+        const int tt = n_tokens == 1 ? 0 : divide(j, p.by_half);
+        const double turns = double(p.positions[t0 + tt]) * p.inv_turns[j - tt * half];
+        float s, c;
+        sincospif(2.f * float(turns - rint(turns)), &s, &c);
+        s_turn[j] = make_float2(c, s);
+      }
+    }
+    __syncthreads();
+  };
 
   // kAhead rows of one kind, from item i0 (token of the block * rows + row) in steps of kGroups
-  auto walk = [&](auto kind_, auto ahead_, const T* src, int64_t tok_stride, int64_t head_stride, int rows, const void* weight) {
+  auto walk = [&](auto kind_, auto ahead_, const T* src, int tok_stride, int head_stride, int rows, unsigned by_rows,
+                  const void* weight) {
     constexpr int kKind = decltype(kind_)::value, kAhead = decltype(ahead_)::value;
     constexpr bool kNormed = kNorm && kKind != kRowV;
     const int items = n_tokens * rows;
-    src += t0 * tok_stride + at;
+    src += (long long)t0 * tok_stride + at;
+    T* out_rows = static_cast<T*>(kKind == kRowQ ? p.q_out : kKind == kRowK ? p.k_out : nullptr);
+    if (out_rows) out_rows += (long long)t0 * rows * p.dim + at;
     float w[8];
     for (int i0 = group; i0 - group < items; i0 += kGroups * kAhead) {      // the lanes of a warp stay together
       uint4 raw[kAhead];
 #pragma unroll
       for (int a = 0; a < kAhead; ++a) {
         const int item = i0 + a * kGroups;
-        const int tt = n_tokens == 1 ? 0 : item / rows, r = item - tt * rows;
-        raw[a] = item < items && active ? load_row<T, kSplit>(src + tt * tok_stride + r * head_stride, half)
-                                        : make_uint4(0u, 0u, 0u, 0u);
+        raw[a] = make_uint4(0u, 0u, 0u, 0u);
+        if (item < items && active) {
+          const int tt = n_tokens == 1 ? 0 : divide(item, by_rows), r = item - tt * rows;
+          raw[a] = load_row<T, kSplit>(src + (long long)tt * tok_stride + (long long)r * head_stride, half);
+        }
       }
       if constexpr (kNormed) {
         if (i0 == group) load_weight8<T>(weight, p.weight_f32, at, at2, active, w);
-        if (!ready) {        // the angles, while the first rows are on their way
-          ready = true;
-          for (int j = threadIdx.x; j < n_tokens * half; j += kThreads) {
-            const int tt = n_tokens == 1 ? 0 : j / half;
-            const double turns = double(p.positions[t0 + tt]) * p.inv_turns[j - tt * half];
-            float s, c;
-            sincospif(2.f * float(turns - rint(turns)), &s, &c);
-            s_turn[j] = make_float2(c, s);
-          }
-          __syncthreads();
-        }
+      }
+      if (!ready) {
+        ready = true;
+        prepare();
       }
 #pragma unroll
       for (int a = 0; a < kAhead; ++a) {
         const int item = i0 + a * kGroups;
         if (item - group >= items) break;          // the same for the whole block
-        const int tt = n_tokens == 1 ? 0 : item / rows, r = item - tt * rows;
-        const bool live = item < items;
+        const bool live = item < items;            // a group behind the last row only takes part in the shuffles
+        const int tt = n_tokens == 1 || !live ? 0 : divide(item, by_rows), r = live ? item - tt * rows : 0;
         uint4 out = raw[a];
         if constexpr (kNormed) {
           float x[8];
@@ -183,40 +218,30 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(RowsParams p) {
           }
           out = pack8<T>(x);
         }
-        const int t = t0 + tt;
-        if constexpr (kKind == kRowQ) {
-          if (live && active)
-            store_row<T, kSplit>(static_cast<T*>(p.q_out) + (size_t(t) * p.heads + r) * p.dim + at, half, out);
-        } else {
-          if (kKind == kRowK && p.k_out && live && active)
-            store_row<T, kSplit>(static_cast<T*>(p.k_out) + (size_t(t) * p.heads_kv + r) * p.dim + at, half, out);
-          if constexpr (kCache != kNoCache) {
-            const int slot = live ? __ldg(p.slots + t) : -1;
-            const bool stored = slot >= 0 && slot < p.pool_tokens;
-            if constexpr (kCache == kCache16) {
-              if (stored && active)
-                store_row<T, kSplit>(static_cast<T*>(kKind == kRowK ? p.k_cache : p.v_cache) +
-                                         (size_t(slot) * p.heads_kv + r) * p.dim + at, half, out);
+        if (out_rows && live && active) store_row<T, kSplit>(out_rows + (long long)item * p.dim, half, out);
+        if constexpr (kKind != kRowQ && kCache == kCache16) {
+          const long long to = live ? s_to[tt] : -1;
+          if (to >= 0 && active)
+            store_row<T, kSplit>(static_cast<T*>(kKind == kRowK ? p.k_cache : p.v_cache) + to + r * p.dim + at, half, out);
+        }
+        if constexpr (kKind != kRowQ && kCache == kCacheInt4) {
+          const long long to = live ? s_to[tt] : -1;
+          const int tok = live ? s_row[tt] : 0;
+          float z[8];
+          unpack8<T>(out, z);
+          uint32_t params;
+          const uint32_t codes = int4_quantise<kLanes>(z, tok & 1, params);
+          if (to >= 0) {
+            constexpr int part = kKind == kRowK ? 0 : 1;
+            unsigned char* rec = static_cast<unsigned char*>(p.k_cache) + to + r * head_bytes;
+            unsigned char* row = rec + (part * kInt4Tokens + tok) * (p.dim / 2);
+            if constexpr (kSplit) {
+              *reinterpret_cast<uint16_t*>(row + lane * 2) = uint16_t(codes);
+              *reinterpret_cast<uint16_t*>(row + p.dim / 4 + lane * 2) = uint16_t(codes >> 16);
             } else {
-              float z[8];
-              unpack8<T>(out, z);
-              uint32_t params;
-              const uint32_t codes = int4_quantise<kLanes>(z, slot & 1, params);
-              if (stored) {
-                unsigned char* rec = static_cast<unsigned char*>(p.k_cache) +
-                                     int4_record_of(slot, r, p.heads_kv, p.page_size, p.dim);
-                constexpr int part = kKind == kRowK ? 0 : 1;
-                const int tok = slot % kInt4Tokens;
-                unsigned char* row = rec + (part * kInt4Tokens + tok) * (p.dim / 2);
-                if constexpr (kSplit) {
-                  *reinterpret_cast<uint16_t*>(row + lane * 2) = uint16_t(codes);
-                  *reinterpret_cast<uint16_t*>(row + p.dim / 4 + lane * 2) = uint16_t(codes >> 16);
-                } else {
-                  *reinterpret_cast<uint32_t*>(row + lane * 4) = codes;
-                }
-                if (lane == 0) *reinterpret_cast<uint32_t*>(rec + kInt4Tokens * p.dim + tok * 8 + part * 4) = params;
-              }
+              *reinterpret_cast<uint32_t*>(row + lane * 4) = codes;
             }
+            if (lane == 0) *reinterpret_cast<uint32_t*>(rec + kInt4Tokens * p.dim + tok * 8 + part * 4) = params;
           }
         }
       }
@@ -227,10 +252,10 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(RowsParams p) {
   using V = std::integral_constant<int, kRowV>;
   using Ahead = std::integral_constant<int, 4>;
   if constexpr (kNorm)
-    walk(Q{}, Ahead{}, static_cast<const T*>(p.q), p.q_tok, p.q_head, p.heads, p.q_weight);
-  walk(K{}, Ahead{}, static_cast<const T*>(p.k), p.k_tok, p.k_head, p.heads_kv, p.k_weight);
+    walk(Q{}, Ahead{}, static_cast<const T*>(p.q), p.q_tok, p.q_head, p.heads, p.by_heads, p.q_weight);
+  walk(K{}, Ahead{}, static_cast<const T*>(p.k), p.k_tok, p.k_head, p.heads_kv, p.by_heads_kv, p.k_weight);
   if constexpr (kCache != kNoCache)
-    walk(V{}, Ahead{}, static_cast<const T*>(p.v), p.v_tok, p.v_head, p.heads_kv, nullptr);
+    walk(V{}, Ahead{}, static_cast<const T*>(p.v), p.v_tok, p.v_head, p.heads_kv, p.by_heads_kv, nullptr);
 }
 
 template <typename T, int kLanes, int kCache, bool kNorm>
@@ -238,13 +263,21 @@ void launch_lanes(RowsParams p, int tokens, cudaStream_t s) {
   constexpr int kGroups = kThreads / kLanes;
   p.tokens = tokens;
   p.inv_dim = 1.f / float(p.dim);
+  p.by_heads = reciprocal(p.heads);
+  p.by_heads_kv = reciprocal(p.heads_kv);
+  p.by_half = reciprocal(p.rotary_dim / 2);
   // about kRowsPerGroup rows for every group of lanes, however few heads there are
-  constexpr int kRowsPerGroup = 6;
+#ifndef TB200_ROWS_PER_GROUP
+#define TB200_ROWS_PER_GROUP 12
+#endif
+  constexpr int kRowsPerGroup = TB200_ROWS_PER_GROUP;
   p.block_tokens = kRowsPerGroup * kGroups / p.rows;
   if (p.block_tokens < 1) p.block_tokens = 1;
   if (p.block_tokens > kMaxTokens) p.block_tokens = kMaxTokens;
-  // few tokens: one to a block, so that they spread over the SMs
-  if (tokens < sm_count() * 4) p.block_tokens = 1;
+  // but three blocks for every SM where there are as many tokens (with the 4-bit append and read-back of 2047 tokens of 16 / 4
+  // heads x 64: 10 us in 512 blocks, 11 in 256, 17 in 2047; 8192 of 32 / 8 heads x 128 into a 16-bit cache: 41 us with two
+  // tokens a block, 46 with one)
+  while (p.block_tokens > 1 && tokens / p.block_tokens < sm_count() * 3) --p.block_tokens;
   const int blocks = (tokens + p.block_tokens - 1) / p.block_tokens;
   const size_t smem = kNorm ? size_t(p.block_tokens) * (p.rotary_dim / 2) * sizeof(float2) : 0;
   if (kNorm && p.rotary_dim == p.dim && p.dim % 16 == 0)
@@ -266,6 +299,8 @@ void launch_rows(const RowsParams& p, int tokens, cudaStream_t s) {
 bool aligned_rows(const void* base, int64_t tok, int64_t head) {
   return (reinterpret_cast<uintptr_t>(base) & 15) == 0 && tok % 8 == 0 && head % 8 == 0;
 }
+bool fits_int(int64_t stride) { return stride >= -0x7fffffffLL && stride <= 0x7fffffffLL; }
+constexpr int kMaxHeads = 4096;     // (token, row) pairs of a block are divided in 16 bits
 
 }  // namespace
 }  // namespace tb200
@@ -304,14 +339,18 @@ extern "C" int tb200_qk_norm_rope(const void* q, const void* k, const void* v, v
       (cache != TB200_CACHE_NONE && (!aligned_rows(v, v_token_stride, v_head_stride) || !aligned_rows(k_cache, 0, 0) ||
                                      !aligned_rows(v_cache, 0, 0))))
     TB200_FAIL(TB200_ERR_UNSUPPORTED, "rows must start on 16-byte boundaries");
+  if (heads > kMaxHeads || heads_kv > kMaxHeads) TB200_FAIL(TB200_ERR_UNSUPPORTED, "at most %d heads", kMaxHeads);
+  if (!fits_int(q_token_stride) || !fits_int(q_head_stride) || !fits_int(k_token_stride) || !fits_int(k_head_stride) ||
+      !fits_int(v_token_stride) || !fits_int(v_head_stride))
+    TB200_FAIL(TB200_ERR_UNSUPPORTED, "strides must fit 32 bits");
   RowsParams p{};
   p.q = q; p.k = k; p.v = v; p.q_out = q_out; p.k_out = k_out;
   p.q_weight = q_weight; p.k_weight = k_weight; p.weight_f32 = weight_dtype == TB200_F32;
   p.inv_turns = inv_turns; p.positions = positions; p.slots = slots; p.k_cache = k_cache; p.v_cache = v_cache;
   p.heads = heads; p.heads_kv = heads_kv; p.dim = dim; p.rotary_dim = rotary_dim; p.page_size = page_size;
   p.rows = heads + heads_kv + (cache != TB200_CACHE_NONE ? heads_kv : 0);
-  p.q_tok = q_token_stride; p.q_head = q_head_stride; p.k_tok = k_token_stride; p.k_head = k_head_stride;
-  p.v_tok = v_token_stride; p.v_head = v_head_stride;
+  p.q_tok = int(q_token_stride); p.q_head = int(q_head_stride); p.k_tok = int(k_token_stride);
+  p.k_head = int(k_head_stride); p.v_tok = int(v_token_stride); p.v_head = int(v_head_stride);
   p.pool_tokens = int(pool_tokens); p.eps = eps;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == TB200_BF16) {
@@ -342,10 +381,13 @@ extern "C" int tb200_int4_cache_append(const void* k, const void* v, const int32
   if (!aligned_rows(k, k_token_stride, k_head_stride) || !aligned_rows(v, v_token_stride, v_head_stride) ||
       !aligned_rows(kv_pages, 0, 0))
     TB200_FAIL(TB200_ERR_UNSUPPORTED, "rows must start on 16-byte boundaries");
+  if (heads_kv > kMaxHeads) TB200_FAIL(TB200_ERR_UNSUPPORTED, "at most %d heads", kMaxHeads);
+  if (!fits_int(k_token_stride) || !fits_int(k_head_stride) || !fits_int(v_token_stride) || !fits_int(v_head_stride))
+    TB200_FAIL(TB200_ERR_UNSUPPORTED, "strides must fit 32 bits");
   RowsParams p{};
   p.k = k; p.v = v; p.slots = slots; p.k_cache = kv_pages;
   p.heads = 0; p.heads_kv = heads_kv; p.dim = dim; p.page_size = page_size; p.rows = 2 * heads_kv;
-  p.k_tok = k_token_stride; p.k_head = k_head_stride; p.v_tok = v_token_stride; p.v_head = v_head_stride;
+  p.k_tok = int(k_token_stride); p.k_head = int(k_head_stride); p.v_tok = int(v_token_stride); p.v_head = int(v_head_stride);
   p.pool_tokens = int(pool_tokens);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == TB200_BF16) launch_rows<__nv_bfloat16, kCacheInt4, false>(p, tokens, s);

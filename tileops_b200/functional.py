@@ -589,7 +589,8 @@ def _rows(t: torch.Tensor) -> "Tuple[torch.Tensor, int, int]":
     tokens, heads, dim = t.shape
     tok = t.stride(0) if tokens > 1 else heads * dim
     head = t.stride(1) if heads > 1 else dim
-    if (t.stride(2) == 1 or dim == 1) and tok % 8 == 0 and head % 8 == 0 and t.data_ptr() % 16 == 0:
+    if ((t.stride(2) == 1 or dim == 1) and tok % 8 == 0 and head % 8 == 0 and t.data_ptr() % 16 == 0
+            and tok < 1 << 31 and head < 1 << 31):
         return t, tok, head
     return t.clone(memory_format=torch.contiguous_format), heads * dim, dim
 
