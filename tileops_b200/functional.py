@@ -507,6 +507,8 @@ class PagedKVPlan(NamedTuple):
 
 
 def _check_vector(name: str, t: torch.Tensor, n: int, device: torch.device, dtype: torch.dtype = torch.int32) -> None:
+    if t.dtype is dtype and t.shape == (n,) and t.device == device and t.is_contiguous():
+        return
     if t.dtype != dtype or t.dim() != 1 or t.shape[0] != n:
         raise ValueError(f"{name} must be {str(dtype)[6:]} with shape ({n},), got {t.dtype} {tuple(t.shape)}")
     if t.device != device:
@@ -516,6 +518,9 @@ def _check_vector(name: str, t: torch.Tensor, n: int, device: torch.device, dtyp
 
 
 def _check_table(block_table: torch.Tensor, batch: int, device: torch.device) -> None:
+    if (block_table.dtype is torch.int32 and block_table.dim() == 2 and block_table.shape[0] == batch
+            and block_table.device == device and block_table.shape[1] > 0 and block_table.is_contiguous()):
+        return
     if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != batch:
         raise ValueError(f"block_table must be int32 with shape [{batch}, num_pages], got {block_table.dtype} "
                          f"{tuple(block_table.shape)}")
@@ -550,10 +555,8 @@ def paged_kv_plan(seq_lens: torch.Tensor, new_lens: torch.Tensor, block_table: t
         _check_vector("free_count", free_count, 1, device)
     if total < 0:
         raise ValueError("total_tokens must not be negative")
-    pad = -total % 4                                    # the maps start on 16-byte boundaries
-    buf = torch.empty(2 * (total + pad) + 3 * batch + 2, dtype=torch.int32, device=device)
-    slots, _, positions, _, cu, after, granted, count = buf.split_with_sizes(
-        [total, pad, total, pad, batch + 1, batch, batch, 1])
+    buf = seq_lens.new_empty(2 * total + 3 * batch + 2)     # one allocation; the slot map, written most, starts it
+    slots, positions, cu, after, granted, count = buf.split_with_sizes([total, total, batch + 1, batch, batch, 1])
     if inplace:
         after, count = seq_lens, free_count
     if free_count is None:
@@ -587,9 +590,12 @@ def _rows(t: torch.Tensor) -> "Tuple[torch.Tensor, int, int]":
     """``t [tokens, heads, dim]`` with its token and head strides, as it is when its rows start on 16-byte boundaries
     (parts of a fused projection's output do), else a contiguous copy."""
     tokens, heads, dim = t.shape
-    tok = t.stride(0) if tokens > 1 else heads * dim
-    head = t.stride(1) if heads > 1 else dim
-    if ((t.stride(2) == 1 or dim == 1) and tok % 8 == 0 and head % 8 == 0 and t.data_ptr() % 16 == 0
+    tok, head, last = t.stride()
+    if tokens <= 1:
+        tok = heads * dim
+    if heads <= 1:
+        head = dim
+    if ((last == 1 or dim == 1) and tok % 8 == 0 and head % 8 == 0 and t.data_ptr() % 16 == 0
             and tok < 1 << 31 and head < 1 << 31):
         return t, tok, head
     return t.clone(memory_format=torch.contiguous_format), heads * dim, dim
@@ -611,6 +617,11 @@ def int4_cache_views(kv_pages: torch.Tensor, page_size: int, dim: int) -> "Tuple
 
 
 def _check_int4_pool(kv_pages: torch.Tensor, heads_kv: int, dim: int, page_size: int, device: torch.device) -> None:
+    shape = kv_pages.shape
+    if (kv_pages.dtype is torch.uint8 and len(shape) == 3 and shape[1] == heads_kv and page_size > 0 and page_size % 16 == 0
+            and shape[2] == page_size * (dim + 8) and (dim == 128 or dim == 64) and kv_pages.device == device
+            and kv_pages.is_contiguous() and kv_pages.data_ptr() % 16 == 0):
+        return
     if page_size <= 0 or page_size % 16 != 0:
         raise ValueError(f"page_size must be a positive multiple of 16, got {page_size}")
     if dim not in (64, 128):
@@ -626,6 +637,8 @@ def _check_int4_pool(kv_pages: torch.Tensor, heads_kv: int, dim: int, page_size:
 
 
 def _check_kv_rows(k: torch.Tensor, v: torch.Tensor) -> None:
+    if k.dim() == 3 and v.shape == k.shape and v.dtype is k.dtype and v.device == k.device:
+        return
     if k.dim() != 3 or v.shape != k.shape:
         raise ValueError(f"k and v must have the same shape [tokens, heads_kv, dim], got {tuple(k.shape)} and "
                          f"{tuple(v.shape)}")
@@ -696,8 +709,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_
             kind, pool_tokens = N.CACHE_16BIT, k_pages.shape[0]
             k_cache, v_cache = k_pages.data_ptr(), v_pages.data_ptr()
         vs = _rows(v)
-    q_out = torch.empty((T, H, D), dtype=dtype, device=device)
-    k_out = torch.empty((T, Hkv, D), dtype=dtype, device=device) if return_k else None
+    q_out = q.new_empty((T, H, D))
+    k_out = q.new_empty((T, Hkv, D)) if return_k else None
     (q, q_tok, q_head), (k, k_tok, k_head) = _rows(q), _rows(k)
     st = N.launch(device, N.lib().tb200_qk_norm_rope, q.data_ptr(), k.data_ptr(), N.ptr(vs[0]), q_out.data_ptr(),
                   N.ptr(k_out), N.ptr(q_weight), N.ptr(k_weight), N.dtype_code(weight_dtype), N.ptr(inv_turns),
@@ -760,9 +773,10 @@ def int4_cache_gather(kv_pages: torch.Tensor, block_table: torch.Tensor, cu_seql
             raise ValueError(f"k_new and v_new must be [tokens, {Hkv}, {dim}] with dtype {dtype} on {device}")
         k_new, v_new = (t if t.is_contiguous() and t.data_ptr() % 16 == 0
                         else t.clone(memory_format=torch.contiguous_format) for t in (k_new, v_new))
+    given, shape = out, (total, Hkv, dim)
     if out is None:
-        out = tuple(torch.empty((total, Hkv, dim), dtype=dtype, device=device) for _ in range(2))
-    for t in out:
+        out = torch.empty(shape, dtype=dtype, device=device), torch.empty(shape, dtype=dtype, device=device)
+    for t in given or ():
         if tuple(t.shape) != (total, Hkv, dim) or t.dtype != dtype or t.device != device or not t.is_contiguous():
             raise ValueError(f"out must be two contiguous [{total}, {Hkv}, {dim}] tensors with dtype {dtype} on {device}")
     st = N.launch(device, N.lib().tb200_int4_cache_gather, kv_pages.data_ptr(), block_table.data_ptr(),
@@ -777,7 +791,11 @@ def _decode_int4_workspace(device: torch.device, batch: int, heads: int, heads_k
     """Scratch of the 4-bit decode.  Eager calls keep one buffer per (device, stream, shape), as the other decode calls do.
     A call under capture gets one of its own from the graph's pool, cleared by a node of the graph: two graphs, or a
     graph and an eager call, that run at the same time then never share counters."""
-    capturing = torch.cuda.is_current_stream_capturing()
+    if device.index == torch.cuda.current_device():
+        capturing = torch.cuda.is_current_stream_capturing()
+    else:
+        with torch.cuda.device(device):
+            capturing = torch.cuda.is_current_stream_capturing()
     key = (device, torch._C._cuda_getCurrentRawStream(device.index), "decode", batch, heads, heads_kv, dim, "int4")
     ws = None if capturing else _WORKSPACES.get(key)
     if ws is None:
@@ -815,7 +833,7 @@ def gqa_decode_int4(q: torch.Tensor, kv_pages: torch.Tensor, real_seqlen_kv: tor
     if not q.is_contiguous() or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)
     out_dtype = q.dtype if out_dtype is None else out_dtype
-    o = torch.empty((B, H, D), dtype=out_dtype, device=device)
+    o = torch.empty_like(q, dtype=out_dtype)
     lse = torch.empty((B, H), dtype=torch.float32, device=device) if return_lse else None
     if B == 0:
         return (o, lse) if return_lse else o

@@ -135,7 +135,8 @@ class GQADecodePagedInt4Sm100Kernel(Kernel):
 
     def forward(self, Q, kv_pages, real_seqlen_kv, block_table, return_lse: bool = False, out_dtype=None):
         return F.gqa_decode_int4(Q, kv_pages, real_seqlen_kv, block_table, page_size=self.page_size,
-                                 sm_scale=self.sm_scale, softcap=self.softcap, return_lse=return_lse, out_dtype=out_dtype)
+                                 sm_scale=self.sm_scale, softcap=self.softcap, return_lse=return_lse, out_dtype=out_dtype,
+                                 config=self.config)
 
 
 class GQAPrefillPagedInt4CacheSm100Kernel(Kernel):

@@ -956,7 +956,7 @@ class GroupedQueryAttentionDecodePagedFp8KVCacheFwdOp(GroupedQueryAttentionDecod
 
 def _check_int4_pool_shape(kv_pages, heads_kv: int, page_size: int, dim: int, pages: Optional[int] = None) -> None:
     want = (heads_kv, page_size * (dim + 8))
-    if kv_pages.ndim != 3 or tuple(kv_pages.shape[1:]) != want or pages not in (None, kv_pages.shape[0]):
+    if kv_pages.shape[1:] != want or pages not in (None, kv_pages.shape[0]):
         raise ValueError(f"kv_pages must have shape [{'pages' if pages is None else pages}, {want[0]}, {want[1]}], "
                          f"got {tuple(kv_pages.shape)}")
 
@@ -983,7 +983,7 @@ class GroupedQueryAttentionDecodePagedInt4KVCacheFwdOp(GroupedQueryAttentionDeco
         return {"o": tuple(q_shape)}
 
     def forward(self, q, kv_pages, real_seqlen_kv, block_table) -> torch.Tensor:
-        if tuple(q.shape) != (self.batch, self.heads, self.dim):
+        if q.shape != (self.batch, self.heads, self.dim):
             raise ValueError(f"q must have shape {(self.batch, self.heads, self.dim)}, got {tuple(q.shape)}")
         _check_int4_pool_shape(kv_pages, self.heads_kv, self.page_size, self.dim, self.seqlen_kv // self.page_size)
         self.dtype = q.dtype
@@ -999,10 +999,6 @@ class GroupedQueryAttentionDecodePagedInt4KVCacheFwdOp(GroupedQueryAttentionDeco
 
     def _pool_pages(self, kv_pages) -> int:
         return kv_pages.shape[0]
-
-    def eval_roofline(self) -> tuple:
-        from ..perf.formulas import gqa_decode_paged_int4_roofline
-        return gqa_decode_paged_int4_roofline(self)
 
 
 class GroupedQueryAttentionPrefillPagedInt4KVCacheFwdOp(Op):

@@ -40,7 +40,7 @@ _UNRESOLVED = object()
 
 _TORCH_DTYPES = {
     "float16": torch.float16, "bfloat16": torch.bfloat16, "float32": torch.float32,
-    "int32": torch.int32, "int64": torch.int64,
+    "int32": torch.int32, "int64": torch.int64, "uint8": torch.uint8,
 }
 if hasattr(torch, "float8_e4m3fn"):
     _TORCH_DTYPES["float8_e4m3fn"] = torch.float8_e4m3fn

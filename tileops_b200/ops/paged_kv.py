@@ -71,9 +71,9 @@ class PagedKVCachePlanFwdOp(Op):
         return {"paged_kv_plan_kernel": PagedKVPlanSm100Kernel}
 
     def _check(self, seq_lens, block_table) -> None:
-        if tuple(seq_lens.shape) != (self.batch,):
+        if seq_lens.shape != (self.batch,):
             raise ValueError(f"seq_lens must have shape ({self.batch},), got {tuple(seq_lens.shape)}")
-        if tuple(block_table.shape) != (self.batch, self.max_pages_per_req):
+        if block_table.shape != (self.batch, self.max_pages_per_req):
             raise ValueError(f"block_table shape must be ({self.batch}, {self.max_pages_per_req}), "
                              f"got {tuple(block_table.shape)}")
 
@@ -159,9 +159,9 @@ class QKNormRopeFwdOp(Op):
         return turns
 
     def _check(self, q, k) -> None:
-        if q.ndim != 3 or tuple(q.shape[1:]) != (self.heads, self.dim):
+        if q.shape[1:] != (self.heads, self.dim):
             raise ValueError(f"q must have shape [T, {self.heads}, {self.dim}], got {tuple(q.shape)}")
-        if k.ndim != 3 or tuple(k.shape[1:]) != (self.heads_kv, self.dim):
+        if k.shape[1:] != (self.heads_kv, self.dim):
             raise ValueError(f"k must have shape [T, {self.heads_kv}, {self.dim}], got {tuple(k.shape)}")
 
     def forward(self, q, k, q_weight, k_weight, positions) -> tuple:
@@ -234,7 +234,7 @@ class Int4KVCacheAppendFwdOp(Op):
         return {"int4_kv_cache_append_kernel": Int4KVCacheAppendSm100Kernel}
 
     def forward(self, k, v, slot_mapping, kv_pages) -> None:
-        if k.ndim != 3 or tuple(k.shape[1:]) != (self.heads_kv, self.dim):
+        if k.shape[1:] != (self.heads_kv, self.dim):
             raise ValueError(f"k must have shape [T, {self.heads_kv}, {self.dim}], got {tuple(k.shape)}")
         slot = "int4_kv_cache_append_kernel"
         self.get_or_build_kernel(slot, (k, v, slot_mapping, kv_pages),
