@@ -67,6 +67,9 @@ constexpr uint32_t kMid = 0x47804780u;   // 7.5 twice in float16
 #ifndef TB200_INT4_MINRUN
 #define TB200_INT4_MINRUN 4
 #endif
+#ifndef TB200_INT4_SEGCOST
+#define TB200_INT4_SEGCOST 2
+#endif
 #ifndef TB200_INT4_B2_64
 #define TB200_INT4_B2_64 2
 #endif
@@ -79,6 +82,8 @@ constexpr uint32_t kMid = 0x47804780u;   // 7.5 twice in float16
 #ifndef TB200_INT4_B64
 #define TB200_INT4_B64 3
 #endif
+
+constexpr unsigned kSegmentCost = TB200_INT4_SEGCOST;   // tiles' worth of time to begin and end a segment
 
 struct Int4DecodeParams {
   const void* q;
@@ -118,8 +123,9 @@ struct Cfg {
   static constexpr int ml = dump + kWarps * kFrags * 512;                     // [kWarps][NT][4] float4
   static constexpr int bars = ml + kWarps * NT * 64;
   static constexpr int segs = bars + 8 * (2 * kStages + 2 * kItemSlots + 2);  // [kItemSlots] Segment
-  static constexpr int misc = segs + kItemSlots * 64;                         // 16 ints
-  static constexpr int plan = misc + 64;                                      // s_prefix [batch + 1], s_lens [batch]
+  static constexpr int ends = segs + kItemSlots * 64;                         // Segments: the range's first, its last so far, the current
+  static constexpr int misc = ends + 3 * 64;                                  // 20 ints
+  static constexpr int plan = misc + 80;                                      // s_prefix [batch + 1], s_lens [batch]
   static_assert(qslots % 128 == 0 && dump % 16 == 0 && bars % 8 == 0, "layout");
 };
 
@@ -137,9 +143,15 @@ struct alignas(16) Segment {
   int too_long;
 };
 static_assert(sizeof(Segment) <= 64, "a slot of shared memory");
+static_assert(kSegmentCost < TB200_INT4_MINRUN, "no range lies in a gap");
+// Slot of the partial result that range k contributes to the lane that starts at unit lane_start.
+__device__ __forceinline__ int segment_slot(int k, unsigned per, unsigned lane_start) {
+  return 2 * k + (unsigned(k) * per >= lane_start ? 0 : 1);
+}
+// The segment at unit u of a range that ends at range_end.  Lanes lie `gap` units apart.
 __device__ __forceinline__ Segment segment_at(const Int4DecodeParams& p, unsigned u, unsigned range_begin,
-                                              unsigned range_end, int range, unsigned per, const int* s_prefix,
-                                              const int* s_lens) {
+                                              unsigned range_end, int range, unsigned per, unsigned gap,
+                                              const int* s_prefix, const int* s_lens) {
   Segment g;
   const int lanes = p.heads_kv * p.n_hb;
   int lo = 0, hi = p.batch - 1;   // largest b with lanes * prefix[b] <= u
@@ -151,30 +163,27 @@ __device__ __forceinline__ Segment segment_at(const Int4DecodeParams& p, unsigne
   const int len = max(s_lens[lo], 0);
   g.too_long = len > p.capacity;
   g.len = min(len, p.capacity);
-  const unsigned tiles_b = unsigned(s_prefix[lo + 1] - s_prefix[lo]);
-  const unsigned local = u - unsigned(s_prefix[lo]) * unsigned(lanes);
-  const int rem = int(local / tiles_b);
-  const unsigned t = local - unsigned(rem) * tiles_b;
+  const unsigned width = unsigned(s_prefix[lo + 1] - s_prefix[lo]);
+  const unsigned base = unsigned(s_prefix[lo]) * unsigned(lanes);
+  const int rem = int((u - base) / width);
   g.hk = p.n_hb == 1 ? rem : rem / p.n_hb;
   g.hbi = rem - g.hk * p.n_hb;
   g.lane = lo * lanes + rem;
-  g.lane_start = u - t;
-  const unsigned lane_end = g.lane_start + tiles_b;
-  g.next = min(range_end, lane_end);
-  g.tile0 = int(t);
-  g.tile1 = int(t + (g.next - u));
+  g.lane_start = base + unsigned(rem) * width + gap;
+  const unsigned lane_end = g.lane_start + width - gap, begin = max(u, g.lane_start);
+  g.tile0 = int(begin - g.lane_start);
+  g.tile1 = int(min(range_end, lane_end) - g.lane_start);
+  g.next = lane_end + gap < range_end ? lane_end : range_end;     // no tile lies in what the range holds of a gap
   const bool whole = g.lane_start >= range_begin && lane_end <= range_end;
   g.first_range = whole ? range : int(g.lane_start / per);
   g.n_runs = whole ? 1 : int((lane_end - 1) / per) - g.first_range + 1;
-  g.slot = 2 * range + (u == range_begin ? 0 : 1);
+  g.slot = segment_slot(range, per, g.lane_start);
   return g;
 }
-// Slot of the partial result that range k contributes to the lane that starts at unit lane_start.
-__device__ __forceinline__ int segment_slot(int k, unsigned per, unsigned lane_start) {
-  return 2 * k + (unsigned(k) * per >= lane_start ? 0 : 1);
-}
 
-// Tile counts of the sequences: s_prefix[0..batch] = exclusive sums, s_lens = lengths as given.  By the math threads.
+// Units of the sequences: s_prefix[0..batch] = exclusive sums per lane, s_lens = lengths as given.  A lane has its tiles
+// and, where lengths differ, kSegmentCost units in front of them for what it costs to begin and end one.  By the
+// math threads.
 template <int kTile>
 __device__ __forceinline__ void tile_plan(const Int4DecodeParams& p, int tid, int* s_prefix, int* s_lens, int* s_sums,
                                           int* s_ragged) {
@@ -182,7 +191,7 @@ __device__ __forceinline__ void tile_plan(const Int4DecodeParams& p, int tid, in
   const int per = (p.batch + kMathThreads - 1) / kMathThreads;
   const int b0 = tid * per;
   const int first_tiles = (min(max(p.lens[0], 0), p.capacity) + kTile - 1) / kTile;
-  int sum = 0;
+  int sum = 0, live = 0;
   bool ragged = false;
   for (int i = 0; i < per; ++i) {
     const int b = b0 + i;
@@ -192,25 +201,31 @@ __device__ __forceinline__ void tile_plan(const Int4DecodeParams& p, int tid, in
       const int t = (min(max(len, 0), p.capacity) + kTile - 1) / kTile;
       ragged |= t != first_tiles;
       sum += t;
+      live += t > 0;
     }
   }
   ragged = __any_sync(0xffffffffu, ragged);
-  if (lane == 0) s_ragged[warp] = ragged ? 1 : 0;
-  int incl = sum;
+  int incl = sum, incl_live = live;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int n = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += n;
+    const int n = __shfl_up_sync(0xffffffffu, incl, o), m = __shfl_up_sync(0xffffffffu, incl_live, o);
+    if (lane >= o) { incl += n; incl_live += m; }
   }
-  if (lane == 31) s_sums[warp] = incl;
+  if (lane == 31) {
+    s_sums[warp] = incl;
+    s_sums[kWarps + warp] = incl_live;
+    s_ragged[warp] = ragged ? 1 : 0;
+  }
   named_barrier(kMathBarrier, kMathThreads);
-  int run = incl - sum;
-  for (int w = 0; w < warp; ++w) run += s_sums[w];
+  const int gap = (s_ragged[0] | s_ragged[1] | s_ragged[2] | s_ragged[3]) ? int(kSegmentCost) : 0;
+  int run = incl - sum + gap * (incl_live - live);
+  for (int w = 0; w < warp; ++w) run += s_sums[w] + gap * s_sums[kWarps + w];
   for (int i = 0; i < per; ++i) {
     const int b = b0 + i;
     if (b < p.batch) {
       s_prefix[b] = run;
-      run += (min(max(s_lens[b], 0), p.capacity) + kTile - 1) / kTile;
+      const int t = (min(max(s_lens[b], 0), p.capacity) + kTile - 1) / kTile;
+      run += t > 0 ? t + gap : 0;
     }
     if (b == p.batch - 1) s_prefix[p.batch] = run;
   }
@@ -353,7 +368,7 @@ __global__ void __launch_bounds__(kAllThreads, Cfg<D, NT>::kBlocks) gqa_decode_i
   auto bar_item_empty = [&](int s) { return smem_u32(bars + 2 * C::kStages + kItemSlots + s); };
   const uint32_t bar_dump = smem_u32(bars + 2 * C::kStages + 2 * kItemSlots);         // every warp has left its part of a segment
   const uint32_t bar_merged = smem_u32(bars + 2 * C::kStages + 2 * kItemSlots + 1);   // every warp has merged its share of it
-  int* s_misc = reinterpret_cast<int*>(smem + C::misc);    // [0] abort, [2..5] warp sums, [6], [7] tickets, [8..11] ragged
+  int* s_misc = reinterpret_cast<int*>(smem + C::misc);    // [0] abort, [6], [7] tickets, [8..11] ragged, [12..19] sums
   volatile int* s_abort = s_misc;
   int* s_prefix = reinterpret_cast<int*>(smem + C::plan);
   int* s_lens = s_prefix + p.batch + 1;
@@ -373,19 +388,21 @@ __global__ void __launch_bounds__(kAllThreads, Cfg<D, NT>::kBlocks) gqa_decode_i
     s_misc[0] = 0;
     mbar_fence_init();
   }
-  if (warp < kWarps) tile_plan<C::kTile>(p, tid, s_prefix, s_lens, s_misc + 2, s_misc + 8);
+  if (warp < kWarps) tile_plan<C::kTile>(p, tid, s_prefix, s_lens, s_misc + 12, s_misc + 8);
   __syncthreads();
 
-  // Units (tiles) per range: an equal share per block, but no run shorter than kMinRun tiles (a run costs its partial
-  // result's way through memory, and the merge of a lane reads all of them).  Sequences of equal length are cut at whole
-  // lanes, or at equal parts of lanes, where that leaves the blocks busy to within a twentieth: fewer runs to merge.
+  // Units per range: an equal share per block, but no run shorter than kMinRun tiles (a run costs its partial result's way
+  // through memory, and the merge of a lane reads all of them).  Sequences of equal length are cut at whole lanes, or at
+  // equal parts of lanes, where that leaves the blocks busy to within a twentieth: fewer runs to merge.
   const unsigned lanes = unsigned(p.heads_kv) * unsigned(p.n_hb);
   const unsigned total_units = unsigned(s_prefix[p.batch]) * lanes;
+  const bool ragged = s_misc[8] | s_misc[9] | s_misc[10] | s_misc[11];
+  const unsigned gap = ragged ? kSegmentCost : 0;
   unsigned per = max((total_units + gridDim.x - 1) / gridDim.x, unsigned(TB200_INT4_MINRUN));
   if (p.force_chunk > 0) {
-    // never so short that the ranges outnumber the slots of the workspace (2 per range)
-    per = max(unsigned(p.force_chunk), (2u * total_units + unsigned(p.max_slots) - 1) / unsigned(p.max_slots));
-  } else if (!(s_misc[8] | s_misc[9] | s_misc[10] | s_misc[11]) && total_units > 0) {
+    // never so short that the ranges outnumber the slots of the workspace (2 per range), nor that one lies in a gap
+    per = max(max(unsigned(p.force_chunk), gap + 1), (2u * total_units + unsigned(p.max_slots) - 1) / unsigned(p.max_slots));
+  } else if (!ragged && total_units > 0) {
     const unsigned L = unsigned(s_prefix[1]), lanes_total = unsigned(p.batch) * lanes;
     if (lanes_total >= gridDim.x) {
       const unsigned whole = (lanes_total + gridDim.x - 1) / gridDim.x * L;
@@ -393,7 +410,7 @@ __global__ void __launch_bounds__(kAllThreads, Cfg<D, NT>::kBlocks) gqa_decode_i
     } else if (L <= per) {
       per = L;
     } else {
-      for (unsigned k = (L + per - 1) / per, i = 0; k > 1 && i < 4; --k, ++i) {
+      for (unsigned k = min((L + per - 1) / per, gridDim.x / lanes_total), i = 0; k > 1 && i < 4; --k, ++i) {
         const unsigned part = (L + k - 1) / k;
         if (L % part == 0) {
           if (20ull * part <= 21ull * per) per = part;
@@ -419,7 +436,7 @@ __global__ void __launch_bounds__(kAllThreads, Cfg<D, NT>::kBlocks) gqa_decode_i
         int ok = 1;
         if (lane == 0) ok = mbar_wait(bar_item_empty(slot), slot_par ^ 1, s_abort, status, 601, limit, 100) ? 1 : 0;
         if (!__shfl_sync(0xffffffffu, ok, 0)) { alive = false; break; }
-        const Segment d = segment_at(p, u, range_begin, range_end, range, per, s_prefix, s_lens);
+        const Segment d = segment_at(p, u, range_begin, range_end, range, per, gap, s_prefix, s_lens);
         u = d.next;
         if (lane == 0) {
           *reinterpret_cast<Segment*>(smem + C::segs + slot * 64) = d;     // the math warps need not work it out again
@@ -492,6 +509,7 @@ __global__ void __launch_bounds__(kAllThreads, Cfg<D, NT>::kBlocks) gqa_decode_i
 
     float4* s_dump = reinterpret_cast<float4*>(smem + C::dump);
     float4* s_ml = reinterpret_cast<float4*>(smem + C::ml);
+    Segment* s_ends = reinterpret_cast<Segment*>(smem + C::ends);
     bool alive = true;
     // Barriers of the math warps with a bounded wait; every thread arrives, since an arrival releases the arriving
     // thread's own stores only.
@@ -511,15 +529,15 @@ __global__ void __launch_bounds__(kAllThreads, Cfg<D, NT>::kBlocks) gqa_decode_i
     uint32_t stage_par = 0;
     for (int range = blockIdx.x; alive && (unsigned long long)range * per < total_units; range += gridDim.x) {
       const unsigned range_begin = unsigned(range) * per, range_end = min(range_begin + per, total_units);
-      unsigned last_begin = range_begin;     // first unit of the range's last segment
+      bool shared = false;
       for (unsigned u = range_begin; alive && u < range_end; ++round) {
         const int slot = round & 1;
-        last_begin = u;
+        const bool first = u == range_begin;
         if (!mbar_wait(bar_item_full(slot), (round >> 1) & 1, s_abort, status, 602, limit)) { alive = false; break; }
-        const Segment d = *reinterpret_cast<const Segment*>(smem + C::segs + slot * 64);
+        const Segment& d = *reinterpret_cast<const Segment*>(smem + C::segs + slot * 64);
         u = d.next;
-        const int head0 = d.hk * p.group + d.hbi * p.hb;
-        const int n_heads = min(p.hb, p.group - d.hbi * p.hb);
+        const int n_heads = min(p.hb, p.group - d.hbi * p.hb), tile0 = d.tile0, tile1 = d.tile1, len = d.len;
+        if (tid == 0) s_ends[2] = d;         // (of this thread alone)
 
         // ---- q: B fragments of S^T = K Q^T as signed bytes; alpha undoes the scale, beta is scale * sum(q) ----
         uint32_t qf[NT][kKWords][kDigits][2];
@@ -603,7 +621,7 @@ __global__ void __launch_bounds__(kAllThreads, Cfg<D, NT>::kBlocks) gqa_decode_i
           for (int e = 0; e < 4; ++e) wacc[nt][e] = 0.f;
         }
 
-        for (int tile = d.tile0; tile < d.tile1; ++tile) {
+        for (int tile = tile0; tile < tile1; ++tile) {
           if (!mbar_wait(bar_full(stage), stage_par, s_abort, status, 602, limit)) { alive = false; break; }
           const unsigned char* st = smem + C::ring + stage * C::kStageBytes + warp * C::kRec;
           const int tok0 = (tile * C::kRecords + warp) * kInt4Tokens + tau;
@@ -649,7 +667,6 @@ __global__ void __launch_bounds__(kAllThreads, Cfg<D, NT>::kBlocks) gqa_decode_i
                   s[e] = float(dot[j][nt][1][e] * 256 + dot[j][nt][0][e]);
                   if constexpr (kDigits == 3) s[e] = fmaf(float(dot[j][nt][kDigits - 1][e]), 65536.f, s[e]);
                 }
-                const float m0 = 0.f, m1 = 0.f;
                 x[j][nt][0] = fmaf(s[0] * alpha[nt][0], kpa.x, kpa.y * beta[nt][0]);
                 x[j][nt][1] = fmaf(s[1] * alpha[nt][1], kpa.x, kpa.y * beta[nt][1]);
                 x[j][nt][2] = fmaf(s[2] * alpha[nt][0], kpb.x, kpb.y * beta[nt][0]);
@@ -665,13 +682,13 @@ __global__ void __launch_bounds__(kAllThreads, Cfg<D, NT>::kBlocks) gqa_decode_i
                   for (int e = 0; e < 4; ++e) x[j][nt][e] = soft_cap(x[j][nt][e], p.softcap, inv_cap) * kLog2e;
             }
           }
-          if ((tile + 1) * C::kTile > d.len) {
+          if ((tile + 1) * C::kTile > len) {
             // tokens behind the end: whatever their place holds (NaN, or an older tile) stays out of every sum
 #pragma unroll
             for (int j = 0; j < R; ++j) {
 #pragma unroll
               for (int i = 0; i < 2; ++i) {
-                if (tok0 + j * kWarps * kInt4Tokens + 8 * i >= d.len) {
+                if (tok0 + j * kWarps * kInt4Tokens + 8 * i >= len) {
                   vs[j][i] = 0.f;
                   vm[j][i] = 0.f;
 #pragma unroll
@@ -792,6 +809,10 @@ __global__ void __launch_bounds__(kAllThreads, Cfg<D, NT>::kBlocks) gqa_decode_i
           }
         }
         if (!wait_merged()) break;      // the area held the previous segment
+        if (tid == 0) {
+          if (first) s_ends[0] = s_ends[2];
+          s_ends[1] = s_ends[2];
+        }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -807,6 +828,7 @@ __global__ void __launch_bounds__(kAllThreads, Cfg<D, NT>::kBlocks) gqa_decode_i
         }
         mbar_arrive(bar_dump);
         if (!wait_dump()) break;
+        const Segment e = s_ends[1];
 #pragma unroll
         for (int f = warp; f < C::kFrags; f += kWarps) {
           const int nt = f / kKSteps;
@@ -815,28 +837,26 @@ __global__ void __launch_bounds__(kAllThreads, Cfg<D, NT>::kBlocks) gqa_decode_i
 #pragma unroll
           for (int w = 0; w < kWarps; ++w)
             merge_add(a, s_dump[(w * C::kFrags + f) * 32 + lane], s_ml[(w * NT + nt) * 4 + t4]);
-          if (d.n_runs == 1) {
-            emit<D, TO>(p, a, d.b, head0, n_heads, f, lane);
+          if (e.n_runs == 1) {
+            emit<D, TO>(p, a, e.b, e.hk * p.group + e.hbi * p.hb, min(p.hb, p.group - e.hbi * p.hb), f, lane);
           } else {
-            p.part_o[(size_t(d.slot) * C::kFrags + f) * 32 + lane] = a.o;
+            p.part_o[(size_t(e.slot) * C::kFrags + f) * 32 + lane] = a.o;
             if (f % kKSteps == 0 && g8 == 0)
-              p.part_ml[(size_t(d.slot) * NT + nt) * 4 + t4] = make_float4(a.M0, a.L0, a.M1, a.L1);
+              p.part_ml[(size_t(e.slot) * NT + nt) * 4 + t4] = make_float4(a.M0, a.L0, a.M1, a.L1);
           }
         }
+        shared = s_ends[0].n_runs > 1 || e.n_runs > 1;      // (the range's first segment, its last so far)
         mbar_arrive(bar_merged);
       }
       if (!alive) break;
       // ---- end of the range: only its first and last segments can share their lanes with other ranges; the last block to
       //      finish such a lane merges it ----
-      const Segment first = segment_at(p, range_begin, range_begin, range_end, range, per, s_prefix, s_lens);
-      const bool one = last_begin == range_begin;
-      const Segment last = one ? first : segment_at(p, last_begin, range_begin, range_end, range, per, s_prefix, s_lens);
-      if (first.n_runs == 1 && last.n_runs == 1) continue;
+      if (!shared) continue;
       if (!wait_merged()) break;          // every warp's partial results are written
       if (lane == 0 && warp < 2) {        // one thread takes the first segment's ticket, another the last one's
-        const Segment& d = warp == 0 ? first : last;
+        const Segment& d = s_ends[warp];
         int mine = 0;
-        if (d.n_runs > 1 && (warp == 0 || !one)) {
+        if (d.n_runs > 1 && (warp == 0 || d.lane != s_ends[0].lane)) {
           int* at = p.counters + kCounterWords + d.lane;
           int n;
           asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(n) : "l"(at) : "memory");
@@ -852,7 +872,7 @@ __global__ void __launch_bounds__(kAllThreads, Cfg<D, NT>::kBlocks) gqa_decode_i
 #pragma unroll 1
       for (int i = 0; i < 2; ++i) {
         if (!s_misc[6 + i]) continue;
-        const Segment& d = i ? last : first;
+        const Segment d = s_ends[i];
         for (int f = warp; f < C::kFrags; f += kWarps) {
           Merged a;
           merge_begin(a);
@@ -989,7 +1009,7 @@ extern "C" int tb200_gqa_decode_int4(const void* q, const void* kv_pages, void* 
   const long long capacity = (long long)block_table_width * page_size;
   p.capacity = int(capacity < 0x7fff0000LL ? capacity : 0x7fff0000LL);
   // the partition counts tiles in 32 bits (tiles of 64 tokens or more)
-  if ((long long)batch * ((p.capacity + 63) / 64) * heads_kv * L.n_hb >= (1LL << 31))
+  if ((long long)batch * ((p.capacity + 63) / 64 + kSegmentCost) * heads_kv * L.n_hb >= (1LL << 31))
     TB200_FAIL(TB200_ERR_UNSUPPORTED, "batch x table width x heads_kv is too large");
   p.sm_scale = sm_scale; p.softcap = softcap;
   p.force_chunk = (flags >> TB200_DECODE_CHUNK_TILES_SHIFT) & 0xFFFF;
