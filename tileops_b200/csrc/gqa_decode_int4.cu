@@ -65,10 +65,13 @@ constexpr uint32_t kMid = 0x47804780u;   // 7.5 twice in float16
 #define TB200_INT4_B128 3
 #endif
 #ifndef TB200_INT4_MINRUN
-#define TB200_INT4_MINRUN 4
+#define TB200_INT4_MINRUN 4u
 #endif
 #ifndef TB200_INT4_SEGCOST
 #define TB200_INT4_SEGCOST 2
+#endif
+#ifndef TB200_INT4_BATCH
+#define TB200_INT4_BATCH 6
 #endif
 #ifndef TB200_INT4_B2_64
 #define TB200_INT4_B2_64 2
@@ -83,6 +86,7 @@ constexpr uint32_t kMid = 0x47804780u;   // 7.5 twice in float16
 #define TB200_INT4_B64 3
 #endif
 
+constexpr unsigned kMinRun = TB200_INT4_MINRUN;
 constexpr unsigned kSegmentCost = TB200_INT4_SEGCOST;   // tiles' worth of time to begin and end a segment
 
 struct Int4DecodeParams {
@@ -143,28 +147,36 @@ struct alignas(16) Segment {
   int too_long;
 };
 static_assert(sizeof(Segment) <= 64, "a slot of shared memory");
-static_assert(kSegmentCost < TB200_INT4_MINRUN, "no range lies in a gap");
+static_assert(kSegmentCost < kMinRun, "no range lies in a gap");
 // Slot of the partial result that range k contributes to the lane that starts at unit lane_start.
 __device__ __forceinline__ int segment_slot(int k, unsigned per, unsigned lane_start) {
   return 2 * k + (unsigned(k) * per >= lane_start ? 0 : 1);
 }
-// The segment at unit u of a range that ends at range_end.  Lanes lie `gap` units apart.
+// The segment at unit u of a range that ends at range_end.  Lanes lie `gap` units apart; `even` is their width where all
+// sequences have the same number of tiles, else 0.
 __device__ __forceinline__ Segment segment_at(const Int4DecodeParams& p, unsigned u, unsigned range_begin,
-                                              unsigned range_end, int range, unsigned per, unsigned gap,
+                                              unsigned range_end, int range, unsigned per, unsigned gap, unsigned even,
                                               const int* s_prefix, const int* s_lens) {
   Segment g;
   const int lanes = p.heads_kv * p.n_hb;
-  int lo = 0, hi = p.batch - 1;   // largest b with lanes * prefix[b] <= u
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (unsigned(s_prefix[mid]) * unsigned(lanes) <= u) lo = mid; else hi = mid - 1;
+  int lo = 0;
+  unsigned width = even, base;
+  if (even) {
+    lo = int(u / (even * unsigned(lanes)));
+    base = unsigned(lo) * even * unsigned(lanes);
+  } else {
+    int hi = p.batch - 1;   // largest b with lanes * prefix[b] <= u
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (unsigned(s_prefix[mid]) * unsigned(lanes) <= u) lo = mid; else hi = mid - 1;
+    }
+    width = unsigned(s_prefix[lo + 1] - s_prefix[lo]);
+    base = unsigned(s_prefix[lo]) * unsigned(lanes);
   }
   g.b = lo;
   const int len = max(s_lens[lo], 0);
   g.too_long = len > p.capacity;
   g.len = min(len, p.capacity);
-  const unsigned width = unsigned(s_prefix[lo + 1] - s_prefix[lo]);
-  const unsigned base = unsigned(s_prefix[lo]) * unsigned(lanes);
   const int rem = int((u - base) / width);
   g.hk = p.n_hb == 1 ? rem : rem / p.n_hb;
   g.hbi = rem - g.hk * p.n_hb;
@@ -217,7 +229,7 @@ __device__ __forceinline__ void tile_plan(const Int4DecodeParams& p, int tid, in
     s_ragged[warp] = ragged ? 1 : 0;
   }
   named_barrier(kMathBarrier, kMathThreads);
-  const int gap = (s_ragged[0] | s_ragged[1] | s_ragged[2] | s_ragged[3]) ? int(kSegmentCost) : 0;
+  const int gap = (s_ragged[0] | s_ragged[1] | s_ragged[2] | s_ragged[3]) ? int(kSegmentCost) : 0;   // else added later
   int run = incl - sum + gap * (incl_live - live);
   for (int w = 0; w < warp; ++w) run += s_sums[w] + gap * s_sums[kWarps + w];
   for (int i = 0; i < per; ++i) {
@@ -393,30 +405,34 @@ __global__ void __launch_bounds__(kAllThreads, Cfg<D, NT>::kBlocks) gqa_decode_i
 
   // Units per range: an equal share per block, but no run shorter than kMinRun tiles (a run costs its partial result's way
   // through memory, and the merge of a lane reads all of them).  Sequences of equal length are cut at whole lanes, or at
-  // equal parts of lanes, where that leaves the blocks busy to within a twentieth: fewer runs to merge.
-  const unsigned lanes = unsigned(p.heads_kv) * unsigned(p.n_hb);
-  const unsigned total_units = unsigned(s_prefix[p.batch]) * lanes;
+  // equal parts of lanes, without gaps, where that leaves the blocks busy to within a twentieth: fewer runs to merge.
+  const unsigned lanes = unsigned(p.heads_kv) * unsigned(p.n_hb), lanes_total = unsigned(p.batch) * lanes;
   const bool ragged = s_misc[8] | s_misc[9] | s_misc[10] | s_misc[11];
-  const unsigned gap = ragged ? kSegmentCost : 0;
-  unsigned per = max((total_units + gridDim.x - 1) / gridDim.x, unsigned(TB200_INT4_MINRUN));
+  const unsigned L = ragged ? 0 : unsigned(s_prefix[1]);
+  unsigned gap = kSegmentCost, even = L > 0 ? L + gap : 0;
+  unsigned total_units = L > 0 ? even * lanes_total : unsigned(s_prefix[p.batch]) * lanes;
+  unsigned per = max((total_units + gridDim.x - 1) / gridDim.x, kMinRun);
   if (p.force_chunk > 0) {
     // never so short that the ranges outnumber the slots of the workspace (2 per range), nor that one lies in a gap
     per = max(max(unsigned(p.force_chunk), gap + 1), (2u * total_units + unsigned(p.max_slots) - 1) / unsigned(p.max_slots));
-  } else if (!ragged && total_units > 0) {
-    const unsigned L = unsigned(s_prefix[1]), lanes_total = unsigned(p.batch) * lanes;
+  } else if (L > 0) {
+    unsigned share = max((L * lanes_total + gridDim.x - 1) / gridDim.x, kMinRun);
+    unsigned fit = 0;
     if (lanes_total >= gridDim.x) {
-      const unsigned whole = (lanes_total + gridDim.x - 1) / gridDim.x * L;
-      if (20ull * whole <= 21ull * per) per = whole;
-    } else if (L <= per) {
-      per = L;
+      fit = (lanes_total + gridDim.x - 1) / gridDim.x * L;
+    } else if (L <= share) {
+      fit = share = L;
     } else {
-      for (unsigned k = min((L + per - 1) / per, gridDim.x / lanes_total), i = 0; k > 1 && i < 4; --k, ++i) {
+      for (unsigned k = min((L + share - 1) / share, gridDim.x / lanes_total), i = 0; k > 1 && i < 4 && !fit; --k, ++i) {
         const unsigned part = (L + k - 1) / k;
-        if (L % part == 0) {
-          if (20ull * part <= 21ull * per) per = part;
-          break;
-        }
+        if (L % part == 0) fit = part;
       }
+    }
+    if (fit && 20ull * fit <= 21ull * share) {
+      per = fit;
+      gap = 0;
+      even = L;
+      total_units = L * lanes_total;
     }
   }
   const long long limit = p.wait_cycles;
@@ -436,7 +452,7 @@ __global__ void __launch_bounds__(kAllThreads, Cfg<D, NT>::kBlocks) gqa_decode_i
         int ok = 1;
         if (lane == 0) ok = mbar_wait(bar_item_empty(slot), slot_par ^ 1, s_abort, status, 601, limit, 100) ? 1 : 0;
         if (!__shfl_sync(0xffffffffu, ok, 0)) { alive = false; break; }
-        const Segment d = segment_at(p, u, range_begin, range_end, range, per, gap, s_prefix, s_lens);
+        const Segment d = segment_at(p, u, range_begin, range_end, range, per, gap, even, s_prefix, s_lens);
         u = d.next;
         if (lane == 0) {
           *reinterpret_cast<Segment*>(smem + C::segs + slot * 64) = d;     // the math warps need not work it out again
@@ -873,25 +889,33 @@ __global__ void __launch_bounds__(kAllThreads, Cfg<D, NT>::kBlocks) gqa_decode_i
       for (int i = 0; i < 2; ++i) {
         if (!s_misc[6 + i]) continue;
         const Segment d = s_ends[i];
-        for (int f = warp; f < C::kFrags; f += kWarps) {
-          Merged a;
-          merge_begin(a);
-          // ten runs in flight: a long lane cut over all SMs has dozens, and their latency would add up
-          constexpr int kBatch = 10;
+        // A warp merges fragments of one head tile side by side and has the loads of kBatch runs in flight: a long lane cut
+        // over all SMs has dozens, and their latency would add up.
+        constexpr int kSide = kKSteps / kWarps, kBatch = TB200_INT4_BATCH;
+        for (int f0 = warp; f0 < C::kFrags; f0 += kSide * kWarps) {
+          Merged a[kSide];
+#pragma unroll
+          for (int s = 0; s < kSide; ++s) merge_begin(a[s]);
           for (int r0 = 0; r0 < d.n_runs; r0 += kBatch) {
-            float4 o[kBatch], ml[kBatch];
+            float4 o[kBatch][kSide], ml[kBatch];
 #pragma unroll
             for (int i = 0; i < kBatch; ++i) {
               const int r = min(r0 + i, d.n_runs - 1);
               const size_t it = size_t(segment_slot(d.first_range + r, per, d.lane_start));
-              o[i] = __ldcg(p.part_o + (it * C::kFrags + f) * 32 + lane);
-              ml[i] = __ldcg(p.part_ml + (it * NT + f / kKSteps) * 4 + t4);
+              ml[i] = __ldcg(p.part_ml + (it * NT + f0 / kKSteps) * 4 + t4);
+#pragma unroll
+              for (int s = 0; s < kSide; ++s) o[i][s] = __ldcg(p.part_o + (it * C::kFrags + f0 + s * kWarps) * 32 + lane);
             }
 #pragma unroll
             for (int i = 0; i < kBatch; ++i)
-              if (r0 + i < d.n_runs) merge_add(a, o[i], ml[i]);
+              if (r0 + i < d.n_runs) {
+#pragma unroll
+                for (int s = 0; s < kSide; ++s) merge_add(a[s], o[i][s], ml[i]);
+              }
           }
-          emit<D, TO>(p, a, d.b, d.hk * p.group + d.hbi * p.hb, min(p.hb, p.group - d.hbi * p.hb), f, lane);
+          const int head0 = d.hk * p.group + d.hbi * p.hb, n_heads = min(p.hb, p.group - d.hbi * p.hb);
+#pragma unroll
+          for (int s = 0; s < kSide; ++s) emit<D, TO>(p, a[s], d.b, head0, n_heads, f0 + s * kWarps, lane);
         }
       }
       mbar_arrive(bar_merged);            // the tickets' words and the dump area are free again
