@@ -50,44 +50,10 @@ constexpr int kMathBarrier = 1;
 constexpr int kItemSlots = 2;
 constexpr int kCounterWords = 4;     // [0], [1] spare, [2] status, [3] spare; tickets follow
 constexpr int kMaxBatch = 4096;
-constexpr int kSlotsPerBlock = 4;    // partial results per resident block that the workspace holds
+constexpr int kSlotsPerSm = 12;      // partial results that the workspace holds: 2 per range, a range per resident block
 constexpr float kGrow = 8.f;         // a score this much (log2) above the running maximum moves it
 constexpr int kPBits = 7;            // P * vs is scaled to 2^kPBits: 2^(kGrow + kPBits) < 65504
 constexpr uint32_t kMid = 0x47804780u;   // 7.5 twice in float16
-
-#ifndef TB200_INT4_R128
-#define TB200_INT4_R128 2
-#endif
-#ifndef TB200_INT4_S128
-#define TB200_INT4_S128 3
-#endif
-#ifndef TB200_INT4_B128
-#define TB200_INT4_B128 3
-#endif
-#ifndef TB200_INT4_MINRUN
-#define TB200_INT4_MINRUN 4u
-#endif
-#ifndef TB200_INT4_SEGCOST
-#define TB200_INT4_SEGCOST 2
-#endif
-#ifndef TB200_INT4_BATCH
-#define TB200_INT4_BATCH 6
-#endif
-#ifndef TB200_INT4_B2_64
-#define TB200_INT4_B2_64 2
-#endif
-#ifndef TB200_INT4_R64
-#define TB200_INT4_R64 4
-#endif
-#ifndef TB200_INT4_S64
-#define TB200_INT4_S64 3
-#endif
-#ifndef TB200_INT4_B64
-#define TB200_INT4_B64 3
-#endif
-
-constexpr unsigned kMinRun = TB200_INT4_MINRUN;
-constexpr unsigned kSegmentCost = TB200_INT4_SEGCOST;   // tiles' worth of time to begin and end a segment
 
 struct Int4DecodeParams {
   const void* q;
@@ -112,12 +78,14 @@ struct Int4DecodeParams {
 template <int D, int NT>
 struct Cfg {
   static constexpr int kRec = int4_record_bytes(D);
-  static constexpr int R = D == 128 ? TB200_INT4_R128 : TB200_INT4_R64;       // records of a math warp per tile
+  static constexpr int R = 2;                                                 // records of a math warp per tile
   static constexpr int kRecords = kWarps * R;
   static constexpr int kTile = kRecords * kInt4Tokens;                        // tokens per tile
   static constexpr int kStageBytes = kRecords * kRec;
-  static constexpr int kStages = D == 128 ? TB200_INT4_S128 : TB200_INT4_S64;
-  static constexpr int kBlocks = NT == 2 ? (D == 64 ? TB200_INT4_B2_64 : 2) : D == 128 ? TB200_INT4_B128 : TB200_INT4_B64;   // blocks per SM
+  static constexpr int kStages = D == 128 ? 3 : 4;
+  static constexpr int kBlocks = NT == 2 ? 2 : D == 128 ? 3 : 4;              // per SM
+  static constexpr unsigned kMinRun = D == 128 ? 3 : 4;       // tiles of a run, at least
+  static constexpr unsigned kSegmentCost = D == 128 ? 2 : 3;  // tiles' worth of time to begin and end a segment
   static constexpr int kHeads = 8 * NT;
   static constexpr int kQSlotBytes = kHeads * D * 2;
   static constexpr int kFrags = NT * D / 16;             // accumulator fragments of a warp
@@ -130,6 +98,8 @@ struct Cfg {
   static constexpr int ends = segs + kItemSlots * 64;                         // Segments: the range's first, its last so far, the current
   static constexpr int misc = ends + 3 * 64;                                  // 20 ints
   static constexpr int plan = misc + 80;                                      // s_prefix [batch + 1], s_lens [batch]
+  static_assert(kSegmentCost < kMinRun, "no range lies in a gap");
+  static_assert(2 * kBlocks <= kSlotsPerSm, "every range has its slots");
   static_assert(qslots % 128 == 0 && dump % 16 == 0 && bars % 8 == 0, "layout");
 };
 
@@ -147,7 +117,6 @@ struct alignas(16) Segment {
   int too_long;
 };
 static_assert(sizeof(Segment) <= 64, "a slot of shared memory");
-static_assert(kSegmentCost < kMinRun, "no range lies in a gap");
 // Slot of the partial result that range k contributes to the lane that starts at unit lane_start.
 __device__ __forceinline__ int segment_slot(int k, unsigned per, unsigned lane_start) {
   return 2 * k + (unsigned(k) * per >= lane_start ? 0 : 1);
@@ -196,7 +165,7 @@ __device__ __forceinline__ Segment segment_at(const Int4DecodeParams& p, unsigne
 // Units of the sequences: s_prefix[0..batch] = exclusive sums per lane, s_lens = lengths as given.  A lane has its tiles
 // and, where lengths differ, kSegmentCost units in front of them for what it costs to begin and end one.  By the
 // math threads.
-template <int kTile>
+template <int kTile, unsigned kSegmentCost>
 __device__ __forceinline__ void tile_plan(const Int4DecodeParams& p, int tid, int* s_prefix, int* s_lens, int* s_sums,
                                           int* s_ragged) {
   const int lane = tid & 31, warp = tid >> 5;
@@ -400,7 +369,7 @@ __global__ void __launch_bounds__(kAllThreads, Cfg<D, NT>::kBlocks) gqa_decode_i
     s_misc[0] = 0;
     mbar_fence_init();
   }
-  if (warp < kWarps) tile_plan<C::kTile>(p, tid, s_prefix, s_lens, s_misc + 12, s_misc + 8);
+  if (warp < kWarps) tile_plan<C::kTile, C::kSegmentCost>(p, tid, s_prefix, s_lens, s_misc + 12, s_misc + 8);
   __syncthreads();
 
   // Units per range: an equal share per block, but no run shorter than kMinRun tiles (a run costs its partial result's way
@@ -409,14 +378,14 @@ __global__ void __launch_bounds__(kAllThreads, Cfg<D, NT>::kBlocks) gqa_decode_i
   const unsigned lanes = unsigned(p.heads_kv) * unsigned(p.n_hb), lanes_total = unsigned(p.batch) * lanes;
   const bool ragged = s_misc[8] | s_misc[9] | s_misc[10] | s_misc[11];
   const unsigned L = ragged ? 0 : unsigned(s_prefix[1]);
-  unsigned gap = kSegmentCost, even = L > 0 ? L + gap : 0;
+  unsigned gap = C::kSegmentCost, even = L > 0 ? L + gap : 0;
   unsigned total_units = L > 0 ? even * lanes_total : unsigned(s_prefix[p.batch]) * lanes;
-  unsigned per = max((total_units + gridDim.x - 1) / gridDim.x, kMinRun);
+  unsigned per = max((total_units + gridDim.x - 1) / gridDim.x, C::kMinRun);
   if (p.force_chunk > 0) {
     // never so short that the ranges outnumber the slots of the workspace (2 per range), nor that one lies in a gap
     per = max(max(unsigned(p.force_chunk), gap + 1), (2u * total_units + unsigned(p.max_slots) - 1) / unsigned(p.max_slots));
   } else if (L > 0) {
-    unsigned share = max((L * lanes_total + gridDim.x - 1) / gridDim.x, kMinRun);
+    unsigned share = max((L * lanes_total + gridDim.x - 1) / gridDim.x, C::kMinRun);
     unsigned fit = 0;
     if (lanes_total >= gridDim.x) {
       fit = (lanes_total + gridDim.x - 1) / gridDim.x * L;
@@ -891,7 +860,7 @@ __global__ void __launch_bounds__(kAllThreads, Cfg<D, NT>::kBlocks) gqa_decode_i
         const Segment d = s_ends[i];
         // A warp merges fragments of one head tile side by side and has the loads of kBatch runs in flight: a long lane cut
         // over all SMs has dozens, and their latency would add up.
-        constexpr int kSide = kKSteps / kWarps, kBatch = TB200_INT4_BATCH;
+        constexpr int kSide = kKSteps / kWarps, kBatch = 6;
         for (int f0 = warp; f0 < C::kFrags; f0 += kSide * kWarps) {
           Merged a[kSide];
 #pragma unroll
@@ -948,7 +917,7 @@ Int4Layout make_layout(int batch, int heads, int heads_kv, int dim) {
   L.hb = group < 16 ? group : 16;
   L.nt = L.hb <= 8 ? 1 : 2;
   L.n_hb = (group + L.hb - 1) / L.hb;
-  L.max_slots = sm_count() * 3 * kSlotsPerBlock;
+  L.max_slots = sm_count() * kSlotsPerSm;
   auto up = [](size_t x) { return (x + 255) & ~size_t(255); };
   L.counters_bytes = up((kCounterWords + size_t(batch) * heads_kv * L.n_hb) * 4);
   L.part_o_bytes = up(size_t(L.max_slots) * L.nt * 8 * dim * 4);
@@ -1032,8 +1001,8 @@ extern "C" int tb200_gqa_decode_int4(const void* q, const void* kv_pages, void* 
   p.page_size = page_size; p.hb = L.hb; p.n_hb = L.n_hb;
   const long long capacity = (long long)block_table_width * page_size;
   p.capacity = int(capacity < 0x7fff0000LL ? capacity : 0x7fff0000LL);
-  // the partition counts tiles in 32 bits (tiles of 64 tokens or more)
-  if ((long long)batch * ((p.capacity + 63) / 64 + kSegmentCost) * heads_kv * L.n_hb >= (1LL << 31))
+  // the partition counts tiles in 32 bits (tiles of 64 tokens or more, less than 4 for a gap)
+  if ((long long)batch * ((p.capacity + 63) / 64 + 4) * heads_kv * L.n_hb >= (1LL << 31))
     TB200_FAIL(TB200_ERR_UNSUPPORTED, "batch x table width x heads_kv is too large");
   p.sm_scale = sm_scale; p.softcap = softcap;
   p.force_chunk = (flags >> TB200_DECODE_CHUNK_TILES_SHIFT) & 0xFFFF;
