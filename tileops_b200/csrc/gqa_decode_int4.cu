@@ -329,14 +329,18 @@ __device__ __forceinline__ void emit(const Int4DecodeParams& p, const Merged& a,
   }
 }
 
-// T: type of q.  NT: head tiles of 8 (a KV head with 9 to 16 q heads has two).
-template <int D, int NT, typename T, typename TO>
+// T: type of q.  NT: head tiles of 8 (a KV head with 9 to 16 q heads has two).  kPair: at most 4 q heads of a KV head, so
+// that the second four columns of K's product take the second digit of q, and a lane one token's scores of a record, not two.
+template <int D, int NT, bool kPair, typename T, typename TO>
 __global__ void __launch_bounds__(kAllThreads, Cfg<D, NT>::kBlocks) gqa_decode_int4_kernel(Int4DecodeParams p) {
   using C = Cfg<D, NT>;
   constexpr int R = C::R;
   constexpr int kKSteps = D / 16;
   constexpr int kKWords = D / 32;      // 32-bit words of a K row that a lane reads: 8 dims each, one k step of 32
   constexpr int kDigits = std::is_same<T, __half>::value ? 3 : 2;   // signed bytes of a q
+  constexpr int kDots = kPair ? kDigits - 1 : kDigits;              // products they take
+  constexpr int kRows = kPair ? 1 : 2;                              // tokens of a record whose scores a lane has
+  static_assert(!kPair || NT == 1, "four heads are one tile");
   constexpr int kVWords = D / 64;      // of a V row
   extern __shared__ __align__(128) unsigned char smem[];
   const uint32_t sbase = smem_u32(smem);
@@ -488,7 +492,10 @@ __global__ void __launch_bounds__(kAllThreads, Cfg<D, NT>::kBlocks) gqa_decode_i
     const int k_off = tau * (D / 2) + t4 * (D / 8);                        // K row of MMA row g8; + 8 rows for g8 + 8
     const int v_off0 = 8 * D + t4 * (D / 2) + g8 * (D / 16);               // V row of token t4 (k = 2 t4)
     const int v_off1 = 8 * D + (4 + (t4 ^ 3)) * (D / 2) + g8 * (D / 16);   // V row of k = 2 t4 + 1
-    const int par_off = 16 * D + tau * 8;
+    // (kPair) lanes 0 and 1 of a group take token tau of a record and 2 and 3 token tau + 8, of heads 2 (t4 & 1) and the next
+    const bool upper = kPair && t4 >= 2;
+    const int t_head = kPair ? 2 * (t4 & 1) : 2 * t4, my_tau = tau + (upper ? 8 : 0);
+    const int par_off = 16 * D + my_tau * 8;
     const float score_scale = p.softcap > 0.f ? p.sm_scale : p.sm_scale * kLog2e;
     const float inv_cap = p.softcap > 0.f ? 1.f / p.softcap : 0.f;
 
@@ -525,11 +532,11 @@ __global__ void __launch_bounds__(kAllThreads, Cfg<D, NT>::kBlocks) gqa_decode_i
         if (tid == 0) s_ends[2] = d;         // (of this thread alone)
 
         // ---- q: B fragments of S^T = K Q^T as signed bytes; alpha undoes the scale, beta is scale * sum(q) ----
-        uint32_t qf[NT][kKWords][kDigits][2];
+        uint32_t qf[NT][kKWords][kDots][2];
         float alpha[NT][2], beta[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          const int h = nt * 8 + g8;
+          const int h = kPair ? g8 & 3 : nt * 8 + g8;
           uint32_t raw[D / 8];       // 16-bit pairs: this lane's D / 4 dims
           const uint4* qs = reinterpret_cast<const uint4*>(smem + C::qslots + slot * C::kQSlotBytes + (h * D + t4 * (D / 4)) * 2);
 #pragma unroll
@@ -564,16 +571,24 @@ __global__ void __launch_bounds__(kAllThreads, Cfg<D, NT>::kBlocks) gqa_decode_i
 #pragma unroll
             for (int odd = 0; odd < 2; ++odd) {     // dims 0, 2, 4, 6 of a word are its low nibbles, 1, 3, 5, 7 the high ones
               const uint32_t lo = prmt(n[odd], n[2 + odd], 0x5140u), hi = prmt(n[4 + odd], n[6 + odd], 0x5140u);
-              qf[nt][w][0][odd] = prmt(lo, hi, 0x5410u) ^ 0x80808080u;
-              qf[nt][w][1][odd] = prmt(lo, hi, 0x7632u);
+              uint32_t digit[kDigits];
+              digit[0] = prmt(lo, hi, 0x5410u) ^ 0x80808080u;
+              digit[1] = prmt(lo, hi, 0x7632u);
               if constexpr (kDigits == 3) {
-                qf[nt][w][1][odd] ^= 0x80808080u;
+                digit[1] ^= 0x80808080u;
                 // the third byte is 64 + digit, in 7 bits
                 const uint32_t d = prmt(prmt(n[odd], n[2 + odd], 0x0062u), prmt(n[4 + odd], n[6 + odd], 0x0062u), 0x5410u) ^ 0x40404040u;
-                qf[nt][w][kDigits - 1][odd] = (d & 0x7f7f7f7fu) | ((d & 0x40404040u) << 1);
+                digit[kDigits - 1] = (d & 0x7f7f7f7fu) | ((d & 0x40404040u) << 1);
               }
 #pragma unroll
-              for (int digit = 0; digit < kDigits; ++digit) total[digit] = __dp4a(int(qf[nt][w][digit][odd]), 0x01010101, total[digit]);
+              for (int i = 0; i < kDigits; ++i) total[i] = __dp4a(int(digit[i]), 0x01010101, total[i]);
+              if constexpr (kPair) {
+                qf[nt][w][0][odd] = g8 < 4 ? digit[0] : digit[1];
+                if constexpr (kDigits == 3) qf[nt][w][kDots - 1][odd] = digit[kDigits - 1];     // in both halves
+              } else {
+#pragma unroll
+                for (int i = 0; i < kDigits; ++i) qf[nt][w][i][odd] = digit[i];
+              }
             }
           }
           float sum = float(total[1] * 256 + total[0]);
@@ -585,8 +600,8 @@ __global__ void __launch_bounds__(kAllThreads, Cfg<D, NT>::kBlocks) gqa_decode_i
           const float a = (odd_ones & 15u) ? NAN : score_scale * pow2f(-e), bsum = a * sum;
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            alpha[nt][i] = __shfl_sync(0xffffffffu, a, (2 * t4 + i) * 4);
-            beta[nt][i] = __shfl_sync(0xffffffffu, bsum, (2 * t4 + i) * 4);
+            alpha[nt][i] = __shfl_sync(0xffffffffu, a, (t_head + i) * 4);
+            beta[nt][i] = __shfl_sync(0xffffffffu, bsum, (t_head + i) * 4);
           }
         }
         mbar_arrive(bar_item_empty(slot));   // q is in registers (every thread: its own reads)
@@ -609,12 +624,12 @@ __global__ void __launch_bounds__(kAllThreads, Cfg<D, NT>::kBlocks) gqa_decode_i
         for (int tile = tile0; tile < tile1; ++tile) {
           if (!mbar_wait(bar_full(stage), stage_par, s_abort, status, 602, limit)) { alive = false; break; }
           const unsigned char* st = smem + C::ring + stage * C::kStageBytes + warp * C::kRec;
-          const int tok0 = (tile * C::kRecords + warp) * kInt4Tokens + tau;
+          const int tok0 = (tile * C::kRecords + warp) * kInt4Tokens + my_tau;
 
           // ---- S^T = K Q^T on the codes: 16 tokens x 8 heads per record; the records' products interleave, since each
           //      accumulator is a chain of kKWords dependent MMAs ----
-          float x[R][NT][4];           // scores (log2) less the running maximum
-          float vs[R][2], vm[R][2];    // V scale, and value of the middle code 7.5
+          float x[R][NT][2 * kRows];           // scores (log2): two heads of each token
+          float vs[R][kRows], vm[R][kRows];    // V scale, and value of the middle code 7.5
           {
             uint32_t ka[R][kKWords], kb[R][kKWords];
 #pragma unroll
@@ -622,7 +637,7 @@ __global__ void __launch_bounds__(kAllThreads, Cfg<D, NT>::kBlocks) gqa_decode_i
               lds_words<kKWords>(ka[j], (st + j * kWarps * C::kRec) + k_off);
               lds_words<kKWords>(kb[j], (st + j * kWarps * C::kRec) + k_off + 4 * D);
             }
-            int dot[R][NT][kDigits][4];
+            int dot[R][NT][kDots][4];
 #pragma unroll
             for (int w = 0; w < kKWords; ++w) {
 #pragma unroll
@@ -632,30 +647,40 @@ __global__ void __launch_bounds__(kAllThreads, Cfg<D, NT>::kBlocks) gqa_decode_i
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                  for (int digit = 0; digit < kDigits; ++digit)
+                  for (int digit = 0; digit < kDots; ++digit)
                     mma_16832_u8s8(dot[j][nt][digit], a, qf[nt][w][digit], w == 0);
               }
             }
 #pragma unroll
             for (int j = 0; j < R; ++j) {
-              const uint2 pa = *reinterpret_cast<const uint2*>((st + j * kWarps * C::kRec) + par_off);
-              const uint2 pb = *reinterpret_cast<const uint2*>((st + j * kWarps * C::kRec) + par_off + 64);
-              const float2 kpa = f16x2_to_f32x2(pa.x), kpb = f16x2_to_f32x2(pb.x);
-              const float2 vpa = f16x2_to_f32x2(pa.y), vpb = f16x2_to_f32x2(pb.y);
-              vs[j][0] = vpa.x; vs[j][1] = vpb.x;
-              vm[j][0] = fmaf(7.5f, vpa.x, vpa.y); vm[j][1] = fmaf(7.5f, vpb.x, vpb.y);
+              float ks[kRows], km[kRows];
+#pragma unroll
+              for (int i = 0; i < kRows; ++i) {
+                const uint2 params = *reinterpret_cast<const uint2*>((st + j * kWarps * C::kRec) + par_off + 64 * i);
+                const float2 kp = f16x2_to_f32x2(params.x), vp = f16x2_to_f32x2(params.y);
+                ks[i] = kp.x; km[i] = kp.y;
+                vs[j][i] = vp.x; vm[j][i] = fmaf(7.5f, vp.x, vp.y);
+              }
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
-                float s[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  s[e] = float(dot[j][nt][1][e] * 256 + dot[j][nt][0][e]);
-                  if constexpr (kDigits == 3) s[e] = fmaf(float(dot[j][nt][kDigits - 1][e]), 65536.f, s[e]);
+                for (int e = 0; e < 2 * kRows; ++e) {
+                  int n, third = 0;
+                  if constexpr (kPair) {
+                    // this lane's digit of its own token, and the other one, which is what the lane two further on does
+                    // not need
+                    const int own = upper ? dot[j][nt][0][2 + e] : dot[j][nt][0][e];
+                    const int other = __shfl_xor_sync(0xffffffffu, upper ? dot[j][nt][0][e] : dot[j][nt][0][2 + e], 2);
+                    n = own * (upper ? 256 : 1) + other * (upper ? 1 : 256);
+                    if constexpr (kDigits == 3) third = upper ? dot[j][nt][kDots - 1][2 + e] : dot[j][nt][kDots - 1][e];
+                  } else {
+                    n = dot[j][nt][kDots > 1 ? 1 : 0][e] * 256 + dot[j][nt][0][e];
+                    if constexpr (kDigits == 3) third = dot[j][nt][kDots - 1][e];
+                  }
+                  float s = float(n);
+                  if constexpr (kDigits == 3) s = fmaf(float(third), 65536.f, s);
+                  x[j][nt][e] = fmaf(s * alpha[nt][e & 1], ks[e >> 1], km[e >> 1] * beta[nt][e & 1]);
                 }
-                x[j][nt][0] = fmaf(s[0] * alpha[nt][0], kpa.x, kpa.y * beta[nt][0]);
-                x[j][nt][1] = fmaf(s[1] * alpha[nt][1], kpa.x, kpa.y * beta[nt][1]);
-                x[j][nt][2] = fmaf(s[2] * alpha[nt][0], kpb.x, kpb.y * beta[nt][0]);
-                x[j][nt][3] = fmaf(s[3] * alpha[nt][1], kpb.x, kpb.y * beta[nt][1]);
               }
             }
             if (p.softcap > 0.f) {
@@ -664,7 +689,7 @@ __global__ void __launch_bounds__(kAllThreads, Cfg<D, NT>::kBlocks) gqa_decode_i
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                  for (int e = 0; e < 4; ++e) x[j][nt][e] = soft_cap(x[j][nt][e], p.softcap, inv_cap) * kLog2e;
+                  for (int e = 0; e < 2 * kRows; ++e) x[j][nt][e] = soft_cap(x[j][nt][e], p.softcap, inv_cap) * kLog2e;
             }
           }
           if ((tile + 1) * C::kTile > len) {
@@ -672,7 +697,7 @@ __global__ void __launch_bounds__(kAllThreads, Cfg<D, NT>::kBlocks) gqa_decode_i
 #pragma unroll
             for (int j = 0; j < R; ++j) {
 #pragma unroll
-              for (int i = 0; i < 2; ++i) {
+              for (int i = 0; i < kRows; ++i) {
                 if (tok0 + j * kWarps * kInt4Tokens + 8 * i >= len) {
                   vs[j][i] = 0.f;
                   vm[j][i] = 0.f;
@@ -692,12 +717,13 @@ __global__ void __launch_bounds__(kAllThreads, Cfg<D, NT>::kBlocks) gqa_decode_i
             for (int i = 0; i < 2; ++i) {
               mx[nt][i] = -INFINITY;
 #pragma unroll
-              for (int j = 0; j < R; ++j) mx[nt][i] = max3(mx[nt][i], x[j][nt][i], x[j][nt][2 + i]);
+              for (int j = 0; j < R; ++j)
+                mx[nt][i] = kPair ? fmaxf(mx[nt][i], x[j][nt][i]) : max3(mx[nt][i], x[j][nt][i], x[j][nt][2 * (kRows - 1) + i]);
               grow |= mx[nt][i] > m_run[nt][i] + kGrow;
             }
           }
 #pragma unroll
-          for (int j = 0; j < R; ++j) vtop = max3(vtop, fabsf(vs[j][0]), fabsf(vs[j][1]));
+          for (int j = 0; j < R; ++j) vtop = max3(vtop, fabsf(vs[j][0]), fabsf(vs[j][kRows - 1]));
           grow |= vtop > pow2f(v_exp);
           if (__any_sync(0xffffffffu, grow)) {
             const uint32_t bits = __float_as_uint(vtop);
@@ -712,7 +738,7 @@ __global__ void __launch_bounds__(kAllThreads, Cfg<D, NT>::kBlocks) gqa_decode_i
               for (int i = 0; i < 2; ++i) {
                 float m = mx[nt][i];
 #pragma unroll
-                for (int o = 4; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+                for (int o = kPair ? 2 : 4; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
                 m = fmaxf(m_run[nt][i], m);
                 al[i] = fast_exp2(m_run[nt][i] - m);
                 m_run[nt][i] = m;
@@ -734,17 +760,21 @@ __global__ void __launch_bounds__(kAllThreads, Cfg<D, NT>::kBlocks) gqa_decode_i
 #pragma unroll
           for (int j = 0; j < R; ++j) {
             uint32_t pb[NT][2];
-            const float sa = vs[j][0] * v_norm, sb = vs[j][1] * v_norm;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              const float p0 = fast_exp2(x[j][nt][0] - m_run[nt][0]), p1 = fast_exp2(x[j][nt][1] - m_run[nt][1]);
-              const float p2 = fast_exp2(x[j][nt][2] - m_run[nt][0]), p3 = fast_exp2(x[j][nt][3] - m_run[nt][1]);
-              l_run[nt][0] += p0 + p2;
-              l_run[nt][1] += p1 + p3;
-              corr[nt][0] = fmaf(p0, vm[j][0], fmaf(p2, vm[j][1], corr[nt][0]));
-              corr[nt][1] = fmaf(p1, vm[j][0], fmaf(p3, vm[j][1], corr[nt][1]));
-              pb[nt][0] = movmatrix_trans(pack2<__half>(p0 * sa, p1 * sa));
-              pb[nt][1] = movmatrix_trans(pack2<__half>(p2 * sb, p3 * sb));
+#pragma unroll
+              for (int i = 0; i < kRows; ++i) {
+                const float p0 = fast_exp2(x[j][nt][2 * i] - m_run[nt][0]), p1 = fast_exp2(x[j][nt][2 * i + 1] - m_run[nt][1]);
+                l_run[nt][0] += p0;
+                l_run[nt][1] += p1;
+                corr[nt][0] = fmaf(p0, vm[j][i], corr[nt][0]);
+                corr[nt][1] = fmaf(p1, vm[j][i], corr[nt][1]);
+                const float scale = vs[j][i] * v_norm;
+                pb[nt][i] = movmatrix_trans(pack2<__half>(p0 * scale, p1 * scale));
+              }
+              // columns 0..3 now hold tokens 0..7 of the four heads and columns 4..7 tokens 8..15, which the former want too
+              // (what the latter add up is not used)
+              if constexpr (kPair) pb[nt][1] = __shfl_xor_sync(0xffffffffu, pb[nt][0], 16);
               const uint32_t mid[4] = {kMid, kMid, kMid, kMid};
               mma_16816<__half>(wacc[nt], mid, pb[nt]);
             }
@@ -786,7 +816,7 @@ __global__ void __launch_bounds__(kAllThreads, Cfg<D, NT>::kBlocks) gqa_decode_i
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
 #pragma unroll
-            for (int o = 4; o < 32; o <<= 1) {
+            for (int o = kPair ? 2 : 4; o < 32; o <<= 1) {
               l_run[nt][i] += __shfl_xor_sync(0xffffffffu, l_run[nt][i], o);
               corr[nt][i] += __shfl_xor_sync(0xffffffffu, corr[nt][i], o);
             }
@@ -925,9 +955,9 @@ Int4Layout make_layout(int batch, int heads, int heads_kv, int dim) {
   return L;
 }
 
-template <int D, int NT, typename T, typename TO>
+template <int D, int NT, bool kPair, typename T, typename TO>
 int launch(const Int4DecodeParams& p, cudaStream_t stream) {
-  auto kern = gqa_decode_int4_kernel<D, NT, T, TO>;
+  auto kern = gqa_decode_int4_kernel<D, NT, kPair, T, TO>;
   const size_t smem = smem_bytes<D, NT>(p.batch);
   static thread_local size_t configured[64] = {0}, sized_for[64] = {0};
   static thread_local int resident[64] = {0};
@@ -951,7 +981,8 @@ int launch(const Int4DecodeParams& p, cudaStream_t stream) {
 }
 template <int D, typename T, typename TO>
 int launch_nt(const Int4DecodeParams& p, int nt, cudaStream_t s) {
-  return nt == 1 ? launch<D, 1, T, TO>(p, s) : launch<D, 2, T, TO>(p, s);
+  if (nt == 2) return launch<D, 2, false, T, TO>(p, s);
+  return p.hb <= 4 ? launch<D, 1, true, T, TO>(p, s) : launch<D, 1, false, T, TO>(p, s);
 }
 template <int D, typename T>
 int launch_o(const Int4DecodeParams& p, int nt, int o_dtype, cudaStream_t s) {
