@@ -21,6 +21,8 @@
 // A row that holds a NaN gets NaN parameters: its values, and the outputs that attend to it, are NaN.
 #pragma once
 
+#include <type_traits>
+
 #include "tb200_common.cuh"
 
 namespace tb200 {
@@ -48,23 +50,50 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return y;
 }
 
-// Quantises 8 values of a row that kLanes neighbouring lanes hold together (8 values per lane, all lanes of the group
-// active).  Returns the 8 codes as 4 bytes; `params` (scale in the low half, offset in the high half) is the same on every
+// the same of two 16-bit values side by side
+template <typename T>
+__device__ __forceinline__ uint32_t min2_nan(uint32_t a, uint32_t b) {
+  uint32_t y;
+  if constexpr (std::is_same<T, __half>::value) asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
+  else asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
+  return y;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b) {
+  uint32_t y;
+  if constexpr (std::is_same<T, __half>::value) asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
+  else asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
+  return y;
+}
+
+// Quantises a row that kLanes neighbouring lanes hold together (8 16-bit values per lane, all lanes of the group active).
+// Returns the lane's 8 codes as 4 bytes; `params` (scale in the low half, offset in the high half) is the same on every
 // lane of the group.  Values beyond the clamp need no clamp of their own: their code lies beyond 0 or 15 and is clamped.
 // A code becomes an integer by adding 1.5 * 2^23 (round to nearest even, as rint), and the eight are put together by
 // multiply-adds modulo 2^32, from which the constants' sum is taken off: the conversion and shift units stay free.
-template <int kLanes>
-__device__ __forceinline__ uint32_t int4_quantise(const float (&x)[8], bool odd_slot, uint32_t& params) {
-  float lo = min_nan(min_nan(min_nan(x[0], x[1]), min_nan(x[2], x[3])), min_nan(min_nan(x[4], x[5]), min_nan(x[6], x[7])));
-  float hi = max_nan(max_nan(max_nan(x[0], x[1]), max_nan(x[2], x[3])), max_nan(max_nan(x[4], x[5]), max_nan(x[6], x[7])));
+template <typename T, int kLanes>
+__device__ __forceinline__ uint32_t int4_quantise(uint4 raw, bool odd_slot, uint32_t& params) {
+  // smallest and (negated) largest value side by side
+  const uint32_t small = min2_nan<T>(min2_nan<T>(raw.x, raw.y), min2_nan<T>(raw.z, raw.w));
+  const uint32_t large = max2_nan<T>(max2_nan<T>(raw.x, raw.y), max2_nan<T>(raw.z, raw.w)) ^ 0x80008000u;
+  uint32_t ends = min2_nan<T>(__byte_perm(small, large, 0x5410), __byte_perm(small, large, 0x7632));
 #pragma unroll
-  for (int o = 1; o < kLanes; o <<= 1) {
-    lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+  for (int o = 1; o < kLanes; o <<= 1) ends = min2_nan<T>(ends, __shfl_xor_sync(0xffffffffu, ends, o));
+  const float2 both = unpack2<T>(ends);
+  float lo = both.x, hi = -both.y;
+  float x[8];
+  {
+    const float2 a = unpack2<T>(raw.x), b = unpack2<T>(raw.y), c = unpack2<T>(raw.z), d = unpack2<T>(raw.w);
+    x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y; x[4] = c.x; x[5] = c.y; x[6] = d.x; x[7] = d.y;
   }
   lo = min_nan(max_nan(lo, -kInt4Clamp), kInt4Clamp);
   hi = min_nan(max_nan(hi, -kInt4Clamp), kInt4Clamp);
-  const __half step = __float2half_rn(__fdiv_rn(hi - lo, 15.f));
+  // (hi - lo) / 15, correctly rounded: Markstein's step with the correctly rounded 1 / 15 (where it underflows the float16
+  // is 0 either way)
+  const float span = hi - lo;
+  constexpr float kFifteenth = 1.f / 15.f;
+  const float rough = __fmul_rn(span, kFifteenth);
+  const __half step = __float2half_rn(fmaf(fmaf(-15.f, rough, span), kFifteenth, rough));
   const __half scale = odd_slot ? __hneg(step) : step;
   const __half offset = __float2half_rn(odd_slot ? hi : lo);
   const float s = __half2float(scale), m = __half2float(offset);

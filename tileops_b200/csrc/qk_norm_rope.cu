@@ -227,10 +227,8 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(RowsParams p) {
         if constexpr (kKind != kRowQ && kCache == kCacheInt4) {
           const long long to = live ? s_to[tt] : -1;
           const int tok = live ? s_row[tt] : 0;
-          float z[8];
-          unpack8<T>(out, z);
           uint32_t params;
-          const uint32_t codes = int4_quantise<kLanes>(z, tok & 1, params);
+          const uint32_t codes = int4_quantise<T, kLanes>(out, tok & 1, params);
           if (to >= 0) {
             constexpr int part = kKind == kRowK ? 0 : 1;
             unsigned char* rec = static_cast<unsigned char*>(p.k_cache) + to + r * head_bytes;
