@@ -359,6 +359,20 @@ def test_fixed_runs_agree_with_the_partition_the_kernel_picks(H, D, page, chunk)
     check(lens, H, 2, D, page, config={"chunk_tiles": chunk}, seed=chunk)
 
 
+@pytest.mark.parametrize("lens,H,Hkv,D", [
+    ([1300] * 60, 8, 8, 64),              # equal lanes, more than blocks, that no whole number per block fits
+    ([700] * 37, 16, 4, 128),             # equal lanes, fewer than blocks
+    ([640] * 8, 8, 4, 128),               # equal lanes that are cut into equal parts
+    ([i % 151 for i in range(200)], 8, 4, 128),       # short lanes, some without a token, several per block
+    ([i * 37 % 400 for i in range(90)], 24, 2, 64),   # the same with two head tiles
+    ([1] * 64 + [3000], 8, 2, 128),       # one long request among very short ones
+    ([60000], 4, 1, 128),                 # one lane cut over all blocks: more runs than a merge has in flight
+    ([60000, 5], 32, 2, 64)])
+def test_every_kind_of_partition(lens, H, Hkv, D):
+    for dtype in (torch.bfloat16, torch.float16):
+        check(lens, H, Hkv, D, 64, dtype, seed=len(lens))
+
+
 def test_many_short_segments_per_block_are_bit_reproducible():
     q, pages, lens, table = make([2000, 1333, 128, 999] * 16, 16, 4, 128, 64, seed=14)
     for chunk in (1, 2, 5):

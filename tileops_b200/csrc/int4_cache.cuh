@@ -31,13 +31,6 @@ constexpr int kInt4Tokens = 16;   // tokens of a record
 __host__ __device__ constexpr int int4_record_bytes(int dim) { return kInt4Tokens * (dim + 8); }
 constexpr float kInt4Clamp = 65504.f;   // largest float16
 
-// First byte of the record that holds `slot`, for one KV head.  (slot >= 0)
-__device__ __forceinline__ size_t int4_record_of(int slot, int head, int heads_kv, int page_size, int dim) {
-  const int page = slot / page_size, off = slot - page * page_size;
-  return ((size_t(page) * heads_kv + head) * size_t(page_size / kInt4Tokens) + off / kInt4Tokens) *
-         size_t(int4_record_bytes(dim));
-}
-
 // min and max that pass a NaN on
 __device__ __forceinline__ float min_nan(float a, float b) {
   float y;

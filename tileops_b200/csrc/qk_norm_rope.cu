@@ -14,7 +14,10 @@
 //
 // HBM bound: every row is read and written once.  A group of lanes holds a row, 8 values each, and requests four rows
 // before it works on the first, while the block's angles are still being computed; where all dims rotate, a lane's values are
-// 4 of the first half and their 4 partners, so that the rotation needs no shuffles.
+// 4 of the first half and their 4 partners, so that the rotation needs no shuffles.  Measured, 8192 tokens of 32 / 8 heads x
+// 128, bf16: with the append to a 16-bit cache 41 us = 4.9 TB/s (copies run at 6.5); the SMs issue 64 % of the time and
+// warps wait for their rows and for the schedulers alike.  The 4-bit append of 11755 tokens of 8 heads takes 28 us = 2.2
+// TB/s: about 200 instructions for 8 values of a row, a third of them for its two parameters.
 #include <type_traits>
 
 #include "int4_cache.cuh"
@@ -265,10 +268,7 @@ void launch_lanes(RowsParams p, int tokens, cudaStream_t s) {
   p.by_heads_kv = reciprocal(p.heads_kv);
   p.by_half = reciprocal(p.rotary_dim / 2);
   // about kRowsPerGroup rows for every group of lanes, however few heads there are
-#ifndef TB200_ROWS_PER_GROUP
-#define TB200_ROWS_PER_GROUP 12
-#endif
-  constexpr int kRowsPerGroup = TB200_ROWS_PER_GROUP;
+  constexpr int kRowsPerGroup = 12;
   p.block_tokens = kRowsPerGroup * kGroups / p.rows;
   if (p.block_tokens < 1) p.block_tokens = 1;
   if (p.block_tokens > kMaxTokens) p.block_tokens = kMaxTokens;
