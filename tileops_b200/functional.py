@@ -506,8 +506,14 @@ class PagedKVPlan(NamedTuple):
     granted: torch.Tensor           # [B], 1 or 0
 
 
+def _fits(t: torch.Tensor, dtype: torch.dtype, shape: tuple, index: int) -> bool:
+    """The short answer of the checks below for a contiguous tensor on GPU ``index``: these calls are short, and so is a decode
+    step.  Where it is no, the check itself says what is wrong, if anything is."""
+    return t.dtype is dtype and t.shape == shape and t.get_device() == index and t.is_contiguous()
+
+
 def _check_vector(name: str, t: torch.Tensor, n: int, device: torch.device, dtype: torch.dtype = torch.int32) -> None:
-    if t.dtype is dtype and t.shape == (n,) and t.device == device and t.is_contiguous():
+    if _fits(t, dtype, (n,), device.index):
         return
     if t.dtype != dtype or t.dim() != 1 or t.shape[0] != n:
         raise ValueError(f"{name} must be {str(dtype)[6:]} with shape ({n},), got {t.dtype} {tuple(t.shape)}")
@@ -518,8 +524,8 @@ def _check_vector(name: str, t: torch.Tensor, n: int, device: torch.device, dtyp
 
 
 def _check_table(block_table: torch.Tensor, batch: int, device: torch.device) -> None:
-    if (block_table.dtype is torch.int32 and block_table.dim() == 2 and block_table.shape[0] == batch
-            and block_table.device == device and block_table.shape[1] > 0 and block_table.is_contiguous()):
+    shape = block_table.shape
+    if len(shape) == 2 and shape[1] > 0 and _fits(block_table, torch.int32, (batch, shape[1]), device.index):
         return
     if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != batch:
         raise ValueError(f"block_table must be int32 with shape [{batch}, num_pages], got {block_table.dtype} "
@@ -617,10 +623,8 @@ def int4_cache_views(kv_pages: torch.Tensor, page_size: int, dim: int) -> "Tuple
 
 
 def _check_int4_pool(kv_pages: torch.Tensor, heads_kv: int, dim: int, page_size: int, device: torch.device) -> None:
-    shape = kv_pages.shape
-    if (kv_pages.dtype is torch.uint8 and len(shape) == 3 and shape[1] == heads_kv and page_size > 0 and page_size % 16 == 0
-            and shape[2] == page_size * (dim + 8) and (dim == 128 or dim == 64) and kv_pages.device == device
-            and kv_pages.is_contiguous() and kv_pages.data_ptr() % 16 == 0):
+    if (page_size > 0 and page_size % 16 == 0 and (dim == 128 or dim == 64) and kv_pages.data_ptr() % 16 == 0
+            and _fits(kv_pages, torch.uint8, (kv_pages.shape[0], heads_kv, page_size * (dim + 8)), device.index)):
         return
     if page_size <= 0 or page_size % 16 != 0:
         raise ValueError(f"page_size must be a positive multiple of 16, got {page_size}")
@@ -637,7 +641,8 @@ def _check_int4_pool(kv_pages: torch.Tensor, heads_kv: int, dim: int, page_size:
 
 
 def _check_kv_rows(k: torch.Tensor, v: torch.Tensor) -> None:
-    if k.dim() == 3 and v.shape == k.shape and v.dtype is k.dtype and v.device == k.device:
+    shape = k.shape
+    if len(shape) == 3 and v.shape == shape and v.dtype is k.dtype and v.get_device() == k.get_device():
         return
     if k.dim() != 3 or v.shape != k.shape:
         raise ValueError(f"k and v must have the same shape [tokens, heads_kv, dim], got {tuple(k.shape)} and "
@@ -646,6 +651,14 @@ def _check_kv_rows(k: torch.Tensor, v: torch.Tensor) -> None:
         raise ValueError(f"v must have the dtype of k, got {v.dtype} and {k.dtype}")
     if v.device != k.device:
         raise ValueError(f"v must be on {k.device}, got {v.device}")
+
+
+def _check_weight(name: str, w: torch.Tensor, dtype: torch.dtype, dim: int, device: torch.device) -> torch.dtype:
+    of = w.dtype
+    if of is not dtype and of is not torch.float32:
+        raise ValueError(f"{name} must have the dtype of q or be torch.float32, got {w.dtype}")
+    _check_vector(name, w, dim, device, of)
+    return of
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_turns: Optional[torch.Tensor], *,
@@ -662,36 +675,38 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_
     launch also stores k and v ``[T,Hkv,D]`` at the rows ``slot_mapping`` (int32 ``[T]``; rows outside the pool are
     skipped, rows of one call must be distinct)."""
     _require_cuda(q=q)
-    if q.dim() != 3 or k.dim() != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
+    q_shape, k_shape = q.shape, k.shape
+    if len(q_shape) != 3 or len(k_shape) != 3 or k_shape[0] != q_shape[0] or k_shape[2] != q_shape[2]:
         raise ValueError(f"q must be [tokens, heads, dim] and k [tokens, heads_kv, dim], got {tuple(q.shape)} and "
                          f"{tuple(k.shape)}")
     device, dtype = q.device, q.dtype
-    if dtype not in (torch.float16, torch.bfloat16):
+    index = device.index
+    if dtype is not torch.bfloat16 and dtype is not torch.float16:
         raise ValueError(f"Expected dtype torch.float16 or torch.bfloat16, got {dtype}")
-    if k.dtype != dtype or k.device != device:
+    if k.dtype is not dtype or k.get_device() != index:
         raise ValueError(f"k must have the dtype and device of q, got {k.dtype} on {k.device}")
-    T, H, D = q.shape
-    Hkv = k.shape[1]
+    T, H, D = q_shape
+    Hkv = k_shape[1]
     _check_vector("positions", positions, T, device)
-    half = 0
+    half, turns = 0, None
     if inv_turns is not None:
-        half = inv_turns.numel()
+        half, turns = inv_turns.numel(), inv_turns.data_ptr()
         _check_vector("inv_turns", inv_turns, half, device, torch.float64)
-    weight_dtype = dtype
-    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w is not None:
-            if w.dtype != dtype and w.dtype != torch.float32:
-                raise ValueError(f"{name} must have the dtype of q or be torch.float32, got {w.dtype}")
-            _check_vector(name, w, D, device, w.dtype)
-            weight_dtype = w.dtype
-    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
-        raise ValueError("q_weight and k_weight must have the same dtype")
-    kind, pool_tokens, k_cache, v_cache, vs = N.CACHE_NONE, 0, None, None, (None, 0, 0)
+    weight_dtype, q_w, k_w = dtype, None, None
+    if q_weight is not None:
+        weight_dtype, q_w = _check_weight("q_weight", q_weight, dtype, D, device), q_weight.data_ptr()
+    if k_weight is not None:
+        k_dtype, k_w = _check_weight("k_weight", k_weight, dtype, D, device), k_weight.data_ptr()
+        if q_weight is not None and k_dtype is not weight_dtype:
+            raise ValueError("q_weight and k_weight must have the same dtype")
+        weight_dtype = k_dtype
+    kind, pool_tokens, k_cache, v_cache, slots, v_at, v_tok, v_head = N.CACHE_NONE, 0, None, None, None, None, 0, 0
     if kv_pages is not None or k_pages is not None:
         if v is None or slot_mapping is None:
             raise ValueError("v and slot_mapping come with a cache")
         _check_kv_rows(k, v)
         _check_vector("slot_mapping", slot_mapping, T, device)
+        slots = slot_mapping.data_ptr()
         if kv_pages is not None:
             if k_pages is not None or v_pages is not None:
                 raise ValueError("kv_pages cannot be combined with k_pages / v_pages")
@@ -700,22 +715,27 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_
         else:
             if v_pages is None:
                 raise ValueError("k_pages and v_pages come together")
-            for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
-                if t.dim() != 3 or tuple(t.shape[1:]) != (Hkv, D) or t.shape[0] != k_pages.shape[0] or t.dtype != dtype:
-                    raise ValueError(f"{name} must be [pool_tokens, {Hkv}, {D}] with dtype {dtype}, got {tuple(t.shape)} "
-                                     f"{t.dtype}")
-                if t.device != device or not t.is_contiguous() or t.data_ptr() % 16:
-                    raise ValueError(f"{name} must be contiguous, on {device}, and start on a 16-byte boundary")
-            kind, pool_tokens = N.CACHE_16BIT, k_pages.shape[0]
-            k_cache, v_cache = k_pages.data_ptr(), v_pages.data_ptr()
-        vs = _rows(v)
-    q_out = q.new_empty((T, H, D))
-    k_out = q.new_empty((T, Hkv, D)) if return_k else None
-    (q, q_tok, q_head), (k, k_tok, k_head) = _rows(q), _rows(k)
-    st = N.launch(device, N.lib().tb200_qk_norm_rope, q.data_ptr(), k.data_ptr(), N.ptr(vs[0]), q_out.data_ptr(),
-                  N.ptr(k_out), N.ptr(q_weight), N.ptr(k_weight), N.dtype_code(weight_dtype), N.ptr(inv_turns),
-                  positions.data_ptr(), N.ptr(slot_mapping), k_cache, v_cache, N.dtype_code(dtype), kind, T, H, Hkv, D,
-                  2 * half, q_tok, q_head, k_tok, k_head, vs[1], vs[2], page_size, pool_tokens, eps)
+            kind, k_cache, v_cache = N.CACHE_16BIT, k_pages.data_ptr(), v_pages.data_ptr()
+            pool = k_pages.shape
+            want = (pool[0], Hkv, D) if len(pool) == 3 else None
+            if not (_fits(k_pages, dtype, want, index) and _fits(v_pages, dtype, want, index)
+                    and (k_cache | v_cache) % 16 == 0):
+                for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
+                    if want is None or tuple(t.shape) != want or t.dtype != dtype:
+                        raise ValueError(f"{name} must be [pool_tokens, {Hkv}, {D}] with dtype {dtype}, got "
+                                         f"{tuple(t.shape)} {t.dtype}")
+                    if t.device != device or not t.is_contiguous() or t.data_ptr() % 16:
+                        raise ValueError(f"{name} must be contiguous, on {device}, and start on a 16-byte boundary")
+            pool_tokens = pool[0]
+        v, v_tok, v_head = _rows(v)
+        v_at = v.data_ptr()
+    q_out = q.new_empty(q_shape)
+    k_out = q.new_empty(k_shape) if return_k else None
+    q, q_tok, q_head = _rows(q)
+    k, k_tok, k_head = _rows(k)
+    st = N.launch(device, N.lib().tb200_qk_norm_rope, q.data_ptr(), k.data_ptr(), v_at, q_out.data_ptr(), N.ptr(k_out), q_w, k_w,
+                  N.dtype_code(weight_dtype), turns, positions.data_ptr(), slots, k_cache, v_cache, N.dtype_code(dtype), kind,
+                  T, H, Hkv, D, 2 * half, q_tok, q_head, k_tok, k_head, v_tok, v_head, page_size, pool_tokens, eps)
     N.check(st, "tb200_qk_norm_rope")
     return (q_out, k_out) if return_k else q_out
 
@@ -728,14 +748,16 @@ def int4_cache_append(k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tens
     must be distinct."""
     _require_cuda(k=k)
     _check_kv_rows(k, v)
-    if k.dtype not in (torch.float16, torch.bfloat16):
-        raise ValueError(f"Expected dtype torch.float16 or torch.bfloat16, got {k.dtype}")
+    device, dtype = k.device, k.dtype
+    if dtype is not torch.bfloat16 and dtype is not torch.float16:
+        raise ValueError(f"Expected dtype torch.float16 or torch.bfloat16, got {dtype}")
     T, Hkv, D = k.shape
-    _check_vector("slot_mapping", slot_mapping, T, k.device)
-    _check_int4_pool(kv_pages, Hkv, D, page_size, k.device)
-    (k, k_tok, k_head), (v, v_tok, v_head) = _rows(k), _rows(v)
-    st = N.launch(k.device, N.lib().tb200_int4_cache_append, k.data_ptr(), v.data_ptr(), slot_mapping.data_ptr(),
-                  kv_pages.data_ptr(), N.dtype_code(k.dtype), T, Hkv, D, page_size, kv_pages.shape[0] * page_size,
+    _check_vector("slot_mapping", slot_mapping, T, device)
+    _check_int4_pool(kv_pages, Hkv, D, page_size, device)
+    k, k_tok, k_head = _rows(k)
+    v, v_tok, v_head = _rows(v)
+    st = N.launch(device, N.lib().tb200_int4_cache_append, k.data_ptr(), v.data_ptr(), slot_mapping.data_ptr(),
+                  kv_pages.data_ptr(), N.dtype_code(dtype), T, Hkv, D, page_size, kv_pages.shape[0] * page_size,
                   k_tok, k_head, v_tok, v_head)
     N.check(st, "tb200_int4_cache_append")
 
