@@ -402,7 +402,8 @@ int tb200_gqa_decode_last_kernel(void);
  *   granted           [batch]          1 or 0
  *   free_pages, free_count, free_count_after all NULL: block_table holds every page already (a host that manages its
  *   pages itself); nothing is allocated or written to it, and every request whose lengths make sense is granted
- * batch <= 4096; max_pages_per_req * page_size <= 2^30; page ids * page_size must stay below 2^31.
+ * batch <= 4096; max_pages_per_req * page_size <= 2^30; total_tokens <= 2^30 (here and in the calls below); page ids *
+ * page_size must stay below 2^31.
  *
  * tb200_paged_kv_release puts the pages of the requests with finished[b] != 0 back on the stack (a request's last
  * page first, never beyond free_capacity) and sets their seq_lens to 0; the table keeps its entries.
@@ -459,7 +460,8 @@ int tb200_qk_norm_rope(const void* q, const void* k, const void* v, void* q_out,
  * gather reads it back: output rows cu_seqlens_kv[b] .. cu_seqlens_kv[b + 1] are request b's tokens 0, 1, ..: all of
  * them from the cache (cache_seqlens NULL), or the first cache_seqlens[b] from the cache and the rest from rows
  * cu_seqlens_new[b] .. of k_new / v_new.  scale * code + offset in fp32, rounded to dtype.  total_tokens bounds the rows
- * (rows at or behind cu_seqlens_kv[batch] are left as they were); a page id outside the pool reads as NaN.
+ * (rows at or behind cu_seqlens_kv[batch] are left as they were); a page id outside the pool reads as NaN, and so does a
+ * row outside 0 .. cu_seqlens_new[batch] - 1, which is the number of rows of k_new and v_new.
  * ------------------------------------------------------------------------- */
 int tb200_int4_cache_append(const void* k, const void* v, const int32_t* slots, void* kv_pages, int dtype, int tokens,
                             int heads_kv, int dim, int page_size, int64_t pool_tokens, int64_t k_token_stride,

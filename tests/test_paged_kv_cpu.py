@@ -153,6 +153,19 @@ def test_abi_refuses_without_touching_a_gpu():
     assert size(0, 8, 2, 64) == 0 and size(1, 7, 2, 64) == 0 and size(1, 8, 2, 96) == 0 and size(4, 32, 8, 128) > 0
 
 
+def test_row_counts_that_32_bits_do_not_hold_are_refused():
+    lib = _native.lib()
+    buf = ctypes.create_string_buffer(4096)
+    p = (ctypes.addressof(buf) + 255) // 256 * 256
+    many = (1 << 30) + 1
+    assert lib.tb200_paged_kv_plan(p, p, p, 4, p, 4, p, p, p, p, p, p, p, 2, 4, 16, many, None) == 2
+    assert b"2^30" in lib.tb200_last_error()
+    assert lib.tb200_qk_norm_rope(p, p, p, p, p, p, p, 1, p, p, p, p, p, 1, 0, many, 2, 2, 64, 64, 128, 64, 128, 64, 128, 64, 16,
+                                  16, 1e-6, None) == 2
+    assert lib.tb200_int4_cache_append(p, p, p, p, 1, many, 1, 64, 16, 16, 64, 64, 64, 64, None) == 2
+    assert lib.tb200_int4_cache_gather(p, p, 1, 1, p, None, None, None, None, p, p, 1, many, 1, 1, 64, 16, 1, None) == 2
+
+
 class _Recorder(Kernel):
     supported_archs = None
     general = True

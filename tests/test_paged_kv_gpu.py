@@ -410,6 +410,22 @@ def test_gather_of_ragged_requests_leaves_the_rest_alone():
     assert nan[cu[4] + 16:cu[4] + 32].all() and int(nan.sum()) == 16
 
 
+def test_gather_reads_no_row_that_the_chunk_does_not_have():
+    D, page, Hkv = 64, 16, 2
+    pages = torch.zeros(4, Hkv, F.int4_page_bytes(page, D), dtype=torch.uint8, device=DEV)
+    table = i32([[0, 1], [2, 3]])
+    new = torch.randn(8, Hkv, D, device=DEV).bfloat16()
+    # request 0: 3 cached and 4 new rows; request 1: its lengths ask for rows behind the chunk's 8
+    k, _ = F.int4_cache_gather(pages, table, i32([0, 7, 20]), 20, dim=D, page_size=page, dtype=torch.bfloat16,
+                               cache_seqlens=i32([3, 5]), cu_seqlens_new=i32([0, 4, 8]), k_new=new, v_new=new)
+    assert (k[:3] == 0).all() and torch.equal(k[3:7], new[:4]) and (k[7:12] == 0).all() and torch.equal(k[12:16], new[4:])
+    assert k[16:].isnan().all()
+    # a negative length asks for rows in front of them
+    k, _ = F.int4_cache_gather(pages, table, i32([0, 7, 20]), 20, dim=D, page_size=page, dtype=torch.bfloat16,
+                               cache_seqlens=i32([0, 5]), cu_seqlens_new=i32([-3, 4, 8]), k_new=new, v_new=new)
+    assert k[:3].isnan().all() and torch.equal(k[3:7], new[:4])
+
+
 def test_calls_on_another_stream_and_in_a_graph():
     T, H, Hkv, D, page = 33, 8, 2, 64, 16
     q, k, v, qw, kw = qkv(T, H, Hkv, D, torch.bfloat16, 1, fused=True)

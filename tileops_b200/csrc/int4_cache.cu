@@ -120,7 +120,8 @@ __global__ void __launch_bounds__(kThreads + 32, kBlocksPerSm) int4_gather_kerne
       }
       const int t = g - p.cu[lo];
       if (p.cached && t >= p.cached[lo]) {
-        src = -3 - ((long long)p.cu_new[lo] + t - p.cached[lo]);
+        const long long from = (long long)p.cu_new[lo] + t - p.cached[lo];
+        src = from >= 0 && from < p.cu_new[p.batch] ? -3 - from : -1;     // a row that k_new does not have reads as NaN
       } else {
         const int column = t / p.page_size, off = t - column * p.page_size;
         const int page = column < p.table_width ? p.table[int64_t(lo) * p.table_stride + column] : -1;
@@ -164,6 +165,7 @@ extern "C" int tb200_int4_cache_gather(const void* kv_pages, const int32_t* bloc
   if (page_size <= 0 || page_size % kInt4Tokens != 0)
     TB200_FAIL(TB200_ERR_UNSUPPORTED, "page_size must be a multiple of 16, got %d", page_size);
   if (pool_pages < 0 || pool_pages > 0x7fffffffLL) TB200_FAIL(TB200_ERR_UNSUPPORTED, "too many pages");
+  if (total_tokens > 1 << 30) TB200_FAIL(TB200_ERR_UNSUPPORTED, "at most 2^30 tokens");    // rows are counted in 32 bits
   if (total_tokens == 0) return TB200_OK;
   if (!kv_pages || !block_table || !cu_seqlens_kv || !k_out || !v_out)
     TB200_FAIL(TB200_ERR_BAD_ARGUMENT, "kv_pages, block_table, cu_seqlens_kv, k_out and v_out must be non-null");

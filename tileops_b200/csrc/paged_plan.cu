@@ -272,6 +272,7 @@ extern "C" int tb200_paged_kv_plan(const int32_t* seq_lens, const int32_t* new_l
                                    int max_pages_per_req, int page_size, int total_tokens, void* stream) {
   if (const int st = check_plan_sizes(batch, max_pages_per_req, page_size, free_capacity)) return st;
   if (total_tokens < 0) TB200_FAIL(TB200_ERR_BAD_ARGUMENT, "total_tokens must not be negative");
+  if (total_tokens > 1 << 30) TB200_FAIL(TB200_ERR_UNSUPPORTED, "at most 2^30 tokens");    // rows are counted in 32 bits
   if (!seq_lens || !new_lens || !block_table || !cu_seqlens || !seq_lens_after || !granted ||
       (free_count && (!free_count_after || (free_capacity > 0 && !free_pages))) ||
       (total_tokens > 0 && (!slots || !positions)))

@@ -327,6 +327,7 @@ extern "C" int tb200_qk_norm_rope(const void* q, const void* k, const void* v, v
       TB200_FAIL(TB200_ERR_UNSUPPORTED, "page_size must be a multiple of 16, got %d", page_size);
   }
   if (pool_tokens < 0 || pool_tokens > 0x7fffffffLL) TB200_FAIL(TB200_ERR_UNSUPPORTED, "the pool must hold fewer than 2^31 tokens");
+  if (tokens > 1 << 30) TB200_FAIL(TB200_ERR_UNSUPPORTED, "at most 2^30 tokens");    // rows are counted in 32 bits
   if (tokens == 0) return TB200_OK;
   if (!q || !k || !q_out || !positions || (rotary_dim > 0 && !inv_turns))
     TB200_FAIL(TB200_ERR_BAD_ARGUMENT, "q, k, q_out, positions and inv_turns must be non-null");
@@ -374,6 +375,7 @@ extern "C" int tb200_int4_cache_append(const void* k, const void* v, const int32
   if (page_size <= 0 || page_size % kInt4Tokens != 0)
     TB200_FAIL(TB200_ERR_UNSUPPORTED, "page_size must be a multiple of 16, got %d", page_size);
   if (pool_tokens < 0 || pool_tokens > 0x7fffffffLL) TB200_FAIL(TB200_ERR_UNSUPPORTED, "the pool must hold fewer than 2^31 tokens");
+  if (tokens > 1 << 30) TB200_FAIL(TB200_ERR_UNSUPPORTED, "at most 2^30 tokens");    // rows are counted in 32 bits
   if (tokens == 0) return TB200_OK;
   if (!k || !v || !slots || !kv_pages) TB200_FAIL(TB200_ERR_BAD_ARGUMENT, "k, v, slots and kv_pages must be non-null");
   if (!aligned_rows(k, k_token_stride, k_head_stride) || !aligned_rows(v, v_token_stride, v_head_stride) ||

@@ -729,8 +729,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_
             pool_tokens = pool[0]
         v, v_tok, v_head = _rows(v)
         v_at = v.data_ptr()
-    q_out = q.new_empty(q_shape)
-    k_out = q.new_empty(k_shape) if return_k else None
+    q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    k_out = torch.empty_like(k, memory_format=torch.contiguous_format) if return_k else None
     q, q_tok, q_head = _rows(q)
     k, k_tok, k_head = _rows(k)
     st = N.launch(device, N.lib().tb200_qk_norm_rope, q.data_ptr(), k.data_ptr(), v_at, q_out.data_ptr(), N.ptr(k_out), q_w, k_w,
@@ -797,7 +797,8 @@ def int4_cache_gather(kv_pages: torch.Tensor, block_table: torch.Tensor, cu_seql
                         else t.clone(memory_format=torch.contiguous_format) for t in (k_new, v_new))
     given, shape = out, (total, Hkv, dim)
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=device), torch.empty(shape, dtype=dtype, device=device)
+        k_out = kv_pages.new_empty(shape, dtype=dtype)
+        out = k_out, torch.empty_like(k_out)
     for t in given or ():
         if tuple(t.shape) != (total, Hkv, dim) or t.dtype != dtype or t.device != device or not t.is_contiguous():
             raise ValueError(f"out must be two contiguous [{total}, {Hkv}, {dim}] tensors with dtype {dtype} on {device}")
@@ -809,15 +810,19 @@ def int4_cache_gather(kv_pages: torch.Tensor, block_table: torch.Tensor, cu_seql
     return out
 
 
+def _capturing(device: torch.device) -> bool:
+    """Is the current stream of ``device`` (which need not be the current one) under capture?"""
+    if device.index == torch.cuda.current_device():
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(device):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def _decode_int4_workspace(device: torch.device, batch: int, heads: int, heads_kv: int, dim: int) -> torch.Tensor:
     """Scratch of the 4-bit decode.  Eager calls keep one buffer per (device, stream, shape), as the other decode calls do.
     A call under capture gets one of its own from the graph's pool, cleared by a node of the graph: two graphs, or a
     graph and an eager call, that run at the same time then never share counters."""
-    if device.index == torch.cuda.current_device():
-        capturing = torch.cuda.is_current_stream_capturing()
-    else:
-        with torch.cuda.device(device):
-            capturing = torch.cuda.is_current_stream_capturing()
+    capturing = _capturing(device)
     key = (device, torch._C._cuda_getCurrentRawStream(device.index), "decode", batch, heads, heads_kv, dim, "int4")
     ws = None if capturing else _WORKSPACES.get(key)
     if ws is None:
@@ -888,7 +893,7 @@ def gqa_prefill_paged_int4_cache(q: torch.Tensor, k_new: torch.Tensor, v_new: to
     slots = paged_kv_plan(cache_seqlens, new_lens, block_table, None, None, total_q, page_size=page_size).slot_mapping
     total_kv = B * block_table.shape[1] * int(page_size)
     key = (device, torch.cuda.current_stream(device).cuda_stream, "int4_cache_packed", total_kv, Hkv, D, q.dtype)
-    capturing = torch.cuda.is_current_stream_capturing()
+    capturing = _capturing(device)
     bufs = None if capturing else _WORKSPACES.get(key)
     if bufs is None:
         bufs = tuple(torch.empty((total_kv, Hkv, D), dtype=q.dtype, device=device) for _ in range(2))
