@@ -31,8 +31,8 @@
 //   * At most four q heads per KV head leave half of N idle: the second digit of q takes it, the lanes of the two halves
 //     exchange what the other needs and have one token's scores of a record each (64 sequences of 512 to 8192 tokens 67.2 ->
 //     63.5 us).
-//   * Three blocks of four math warps per SM (head dim 64: four; two head tiles: two), each with a producer warp that streams records by untiled bulk copies (a whole
-//     tile where the page holds it, else 16 tokens each) into a ring of shared-memory stages, across segment boundaries.
+//   * Three blocks of four math warps per SM (head dim 64: four; two head tiles: two), each with a producer warp that streams records by untiled bulk copies (as many
+//     tokens as a page and a tile have in common, 16 at least) into a ring of shared-memory stages, across segment boundaries.
 //     (One block of twelve math warps, which share every stage and every segment, repeats a segment's beginning and end in
 //     twelve warps instead of four: 157 against 126 us on 128 sequences of 4096 tokens, 8 KV heads.)
 //   * Work is cut into equal contiguous ranges, one per block (stream-K), as in gqa_decode_tma.cu; to begin and end a segment
@@ -73,7 +73,7 @@ struct Int4DecodeParams {
   int table_width, pool_pages, batch, heads, heads_kv, group, page_size;
   int hb, n_hb;            // q heads of a head block, head blocks of a KV head
   int capacity;            // tokens a row of the table can name
-  int records_per_copy;    // 16-token records that one bulk copy fetches: a whole tile's, or 1
+  int records_per_copy;    // 16-token records that one bulk copy fetches: 1, 2, 4, .. a whole tile's
   float sm_scale, softcap;
   int force_chunk, max_slots;
   int* counters;
@@ -444,12 +444,12 @@ __global__ void __launch_bounds__(kAllThreads, Cfg<D, NT>::kBlocks) gqa_decode_i
                     bar_item_full(slot));
         }
         const int32_t* row = p.table + d.b * p.table_stride;
-        const bool whole = p.records_per_copy > 1;
+        const int per_copy = p.records_per_copy;      // (a power of two that divides a page and a tile)
         for (int t0 = d.tile0; t0 < d.tile1 && alive; t0 += kRound) {
-          // this lane's copy of the round: 16 tokens, or (my_rec == 0) all of the tile's live records
+          // this lane's copy of the round: its record and the live ones of the per_copy - 1 behind it
           const int t = t0 + my_tile;
           const int token = (t * C::kRecords + my_rec) * kInt4Tokens;
-          const bool mine = my_tile < kRound && t < d.tile1 && token < d.len && (!whole || my_rec == 0);
+          const bool mine = my_tile < kRound && t < d.tile1 && token < d.len && (my_rec & (per_copy - 1)) == 0;
           const unsigned char* src = nullptr;
           uint32_t bytes = 0;
           bool known = true;
@@ -459,7 +459,7 @@ __global__ void __launch_bounds__(kAllThreads, Cfg<D, NT>::kBlocks) gqa_decode_i
             if (known) {
               src = p.pages + ((size_t(page) * p.heads_kv + d.hk) * size_t(p.page_size / kInt4Tokens) +
                                (token - column * p.page_size) / kInt4Tokens) * size_t(C::kRec);
-              const int n = whole ? min(C::kRecords, (d.len - token + kInt4Tokens - 1) / kInt4Tokens) : 1;
+              const int n = min(per_copy, (d.len - token + kInt4Tokens - 1) / kInt4Tokens);
               bytes = uint32_t(n) * C::kRec;
             }
           }
@@ -475,7 +475,7 @@ __global__ void __launch_bounds__(kAllThreads, Cfg<D, NT>::kBlocks) gqa_decode_i
             if (!all_known) {
               // a page outside the pool: nothing is fetched, and the parameters become NaN, which makes the output NaN
               if (my_tile == i && !known)
-                for (int r = 0; r < (whole ? C::kRecords : 1); ++r)
+                for (int r = 0; r < per_copy; ++r)
                   for (int x = 0; x < kInt4Tokens * 8; x += 4)
                     *reinterpret_cast<uint32_t*>(smem + at + r * C::kRec + kInt4Tokens * D + x) = 0x7e007e00u;
               asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // before a later copy into the same place
@@ -1049,8 +1049,10 @@ extern "C" int tb200_gqa_decode_int4(const void* q, const void* kv_pages, void* 
   p.part_o = reinterpret_cast<float4*>(static_cast<unsigned char*>(workspace) + L.counters_bytes);
   p.part_ml = reinterpret_cast<float4*>(static_cast<unsigned char*>(workspace) + L.counters_bytes + L.part_o_bytes);
   p.wait_cycles = 1000000000LL;   // about 0.5 s
-  const int tile = dim == 128 ? Cfg<128, 1>::kTile : Cfg<64, 1>::kTile;
-  p.records_per_copy = page_size % tile == 0 ? tile / kInt4Tokens : 1;
+  static_assert(Cfg<128, 1>::kRecords == 8 && Cfg<128, 2>::kRecords == 8 && Cfg<64, 1>::kRecords == 8 && Cfg<64, 2>::kRecords == 8,
+                "the copies' sizes");
+  p.records_per_copy = 1;
+  while (p.records_per_copy < 8 && page_size / kInt4Tokens % (2 * p.records_per_copy) == 0) p.records_per_copy *= 2;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (q_dtype == TB200_BF16)
     return dim == 64 ? launch_o<64, __nv_bfloat16>(p, L.nt, o_dtype, s) : launch_o<128, __nv_bfloat16>(p, L.nt, o_dtype, s);
