@@ -39,8 +39,8 @@
 //     counts as two or three tiles (without that 78 us instead of 69 on 64 sequences of 512 to 8192 tokens, whose short lanes
 //     made the blocks that got them late).  Partial results of a (sequence, KV head) that ranges share go to global memory
 //     in accumulator order; the last block to finish merges them, at the end of its range.
-// Measured, 32 q and 8 KV heads x 128, bf16, captured: 8 x 131072 tokens 186 us = 6.1 TB/s (218 us back to back, where the
-// board's power limit takes the clock to 1.65 GHz); 64 sequences of 512 to 8192 tokens 68 us = 4.8 TB/s: of that 6 us pass
+// Measured, 32 q and 8 KV heads x 128, bf16, captured: 8 x 131072 tokens 185 us = 6.2 TB/s (214 us back to back, where the
+// board's power limit takes the clock to 1.65 GHz); 64 sequences of 512 to 8192 tokens 67 us = 4.9 TB/s: of that 6 us pass
 // before the first tile, 5 after the last, and each segment's begin and end cost its block 3; 1 x 1000 tokens 11 us, latency.
 #include <type_traits>
 
