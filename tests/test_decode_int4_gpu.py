@@ -202,6 +202,23 @@ def test_bad_pages_and_lengths_give_nan_and_stay_in_bounds():
 
 
 @pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("page", [32, 48, 64, 128, 256])
+def test_a_bad_page_of_any_size_reaches_its_request_only(page, D):
+    lens = [3 * page + 5, 700, 2 * page, 1]
+    for H in (8, 12):
+        q, pages, t_lens, table = make(lens, H, 2, D, page, seed=page, width=32)
+        want = F.gqa_decode_int4(q, pages, t_lens, table, page_size=page)
+        assert not want.isnan().any()
+        for b, j in ((0, 3), (0, 1), (1, 0), (2, 1), (3, 0)):
+            bad = table.clone()
+            bad[b, j] = pages.shape[0]
+            got = F.gqa_decode_int4(q, pages, t_lens, bad, page_size=page)
+            assert got[b].isnan().all()
+            others = [x for x in range(4) if x != b]
+            assert torch.equal(got[others], want[others])
+
+
+@pytest.mark.parametrize("D", [64, 128])
 def test_nan_in_a_cached_token_reaches_its_heads_only(D):
     q, pages, lens, table = make([50, 300], 8, 2, D, 16, seed=6)
     want = F.gqa_decode_int4(q, pages, lens, table, page_size=16)
