@@ -396,14 +396,14 @@ int tb200_gqa_decode_last_kernel(void);
  *   cu_seqlens        [batch + 1]      exclusive sums of max(new_lens, 0): the packed batch's row ranges
  *   slots, positions  [total_tokens]   row t (request b, its i-th new token): position seq_lens[b] + i and
  *                     block_table[b][position / page_size] * page_size + position % page_size.  Slot -1 in the rows of a
- *                     request that is not granted; slot -1, position 0 in rows behind the last request's
+ *                     request that is not granted, and where the page id is negative or the slot does not fit 32 bits;
+ *                     slot -1, position 0 in rows behind the last request's
  *   seq_lens_after    [batch]          seq + new where granted, else seq; may be seq_lens
  *   free_count_after  [1]              may be free_count
  *   granted           [batch]          1 or 0
  *   free_pages, free_count, free_count_after all NULL: block_table holds every page already (a host that manages its
  *   pages itself); nothing is allocated or written to it, and every request whose lengths make sense is granted
- * batch <= 4096; max_pages_per_req * page_size <= 2^30; total_tokens <= 2^30 (here and in the calls below); page ids *
- * page_size must stay below 2^31.
+ * batch <= 4096; max_pages_per_req * page_size <= 2^30; total_tokens <= 2^30 (here and in the calls below).
  *
  * tb200_paged_kv_release puts the pages of the requests with finished[b] != 0 back on the stack (a request's last
  * page first, never beyond free_capacity) and sets their seq_lens to 0; the table keeps its entries.

@@ -451,3 +451,27 @@ def test_calls_on_another_stream_and_in_a_graph():
     pages.zero_()
     graph.replay()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ---- page ids that the pool does not have ------------------------------------------------------------------------------
+@pytest.mark.parametrize("page", [16, 48, 64])
+@pytest.mark.parametrize("bad", [2 ** 30, -2 ** 31, 2 ** 31 - 1, 2 ** 28, 2 ** 27, -1, -7])
+def test_a_slot_of_a_page_that_32_bits_do_not_hold_is_none(bad, page):
+    """id * page_size is formed in 64 bits: a page that no pool has must not become a row of another one."""
+    old, new = page + 5, 3
+    table = i32([[3, bad], [5, 6]])
+    plan = ops.PagedKVCachePlanFwdOp(2, 2, page)(i32([old, old]), i32([new, new]), table, None, None, 2 * new)
+    slots = plan.slot_mapping.tolist()
+    assert slots[new:] == [6 * page + 5 + i for i in range(new)]
+    fits = bad >= 0 and bad * page + page <= 2 ** 31
+    assert slots[:new] == ([bad * page + 5 + i for i in range(new)] if fits else [-1] * new)
+    # an append to these slots changes no page but its own
+    D, Hkv, pool = 64, 2, 8
+    pages = torch.full((pool, Hkv, F.int4_page_bytes(page, D)), 7, dtype=torch.uint8, device=DEV)
+    k = torch.randn(2 * new, Hkv, D, device=DEV).bfloat16()
+    ops.Int4KVCacheAppendFwdOp(Hkv, D, page)(k, k, plan.slot_mapping, pages)
+    changed = (pages != 7).flatten(1).any(1).nonzero().flatten().tolist()
+    assert changed == [6]
+    # the same from the stack
+    plan = ops.PagedKVCachePlanFwdOp(1, 2, page)(i32([page]), i32([2]), i32([[1, 0]]), i32([4, bad]), i32([2]), 2)
+    assert plan.slot_mapping.tolist() == ([bad * page, bad * page + 1] if fits else [-1, -1])

@@ -7,7 +7,7 @@
 // The j-th new page of a granted request is free_pages[free_count - 1 - (C_b - need_b) - j]: pages come off the top of
 // the stack in the order of the requests, and since C_b never falls, the pages that granted requests take are exactly
 // the top of the stack.  Row t of the packed batch (request b, its i-th new token) sits at position seq_b + i and slot
-// table[b][position / P] * P + position % P.
+// table[b][position / P] * P + position % P, or -1 where the page id is negative or the slot does not fit 32 bits.
 //
 // Without a stack (free_count NULL) the table is taken to hold every page already, and only the maps are built.
 //
@@ -95,7 +95,9 @@ __device__ __forceinline__ void map_row(const PlanParams& p, const PlanShared& s
   const int held = allocates ? (s.seq[lo] + p.page - 1) / p.page : p.width, column = pos / p.page;
   const int id = column < held ? p.table[lo * p.table_stride + column]
                                : p.free_pages[free_count - 1 - s.taken[lo] - (column - held)];
-  slot = id * p.page + (pos - column * p.page);
+  // In 64 bits: a page id that no pool has must not become a row of another page by wrapping.
+  const long long at = (long long)id * p.page + (pos - column * p.page);
+  if (id >= 0 && at <= 0x7fffffffLL) slot = int(at);
 }
 
 __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PlanParams p) {

@@ -547,8 +547,9 @@ def paged_kv_plan(seq_lens: torch.Tensor, new_lens: torch.Tensor, block_table: t
 
     ``total_tokens`` is the number of rows of the packed batch as the host knows it (at least ``sum(new_lens)``).  A
     request whose lengths do not fit the table, or for which the stack is short, is not granted: its rows get slot -1 and
-    it keeps its length.  ``inplace=True`` updates ``seq_lens`` and ``free_count`` themselves (a step that a CUDA graph
-    replays).  With ``free_pages`` and ``free_count`` ``None`` the table is taken to hold every page already."""
+    it keeps its length.  A page id that is negative or too large for a 32-bit slot gives slot -1 too.  ``inplace=True``
+    updates ``seq_lens`` and ``free_count`` themselves (a step that a CUDA graph replays).  With ``free_pages`` and
+    ``free_count`` ``None`` the table is taken to hold every page already."""
     _require_cuda(seq_lens=seq_lens)
     device, batch, total = seq_lens.device, seq_lens.shape[0], int(total_tokens)
     _check_vector("seq_lens", seq_lens, batch, device)

@@ -50,7 +50,8 @@ class PagedKVCachePlanFwdOp(Op):
     Returns a :class:`PagedKVPlan`: ``cu_seqlens_q [B + 1]``, ``slot_mapping`` and ``positions [total_tokens]``, and
     ``seq_lens [B]``, ``free_count [1]`` and ``granted [B]`` after the step.  A request is granted when its lengths fit the
     table and it needs no page or the stack holds enough for it and the requests in front of it; else its rows get slot
-    -1 and it keeps its length.  ``total_tokens`` is the packed batch's row count; rows behind the last request get slot -1
+    -1 and it keeps its length.  A page id that is negative or too large for a 32-bit slot gives slot -1 as well; an append
+    skips slots outside its pool.  ``total_tokens`` is the packed batch's row count; rows behind the last request get slot -1
     and position 0.  ``inplace=True`` updates ``seq_lens`` and ``free_count`` themselves, for a step that a CUDA graph
     replays.  ``free_pages`` and ``free_count`` ``None``: the table holds every page already (the host manages its pages)
     and only the maps are built.  At most 4096 requests.
