@@ -397,3 +397,18 @@ def test_many_short_segments_per_block_are_bit_reproducible():
         for _ in range(60):
             assert torch.equal(F.gqa_decode_int4(q, pages, lens, table, page_size=64, config={"chunk_tiles": chunk}), want)
     assert F.decode_status() == 0
+
+
+@pytest.mark.parametrize("top", [4.1e37, 4.3e37, 1e38, 3.3e38])
+@pytest.mark.parametrize("H,D", [(4, 128), (8, 64), (16, 128)])
+def test_q_up_to_the_largest_bfloat16(H, D, top):
+    """Heads whose largest |q| is near the type's end, with a scale that keeps their scores ordinary."""
+    q, pages, lens, table = make([300, 45], H, 1, D, 16, torch.bfloat16, seed=13)
+    q = (q.double() / q.double().abs().amax(-1, keepdim=True) * top).to(torch.bfloat16)
+    sm_scale = 2.0 ** -124
+    got, lse = F.gqa_decode_int4(q, pages, lens, table, page_size=16, sm_scale=sm_scale, out_dtype=torch.float32, return_lse=True)
+    q, pages, table = q.cpu(), pages.cpu(), table.cpu()
+    ref, ref_lse = O.decode_ref(q, pages, [300, 45], table, 16, sm_scale)
+    to, tl = tolerances(q, pages, [300, 45], table, 16, sm_scale, 0.0)
+    assert ((got.double().cpu() - ref).abs() <= to).all()
+    assert ((lse.double().cpu() - ref_lse).abs() <= tl + ref_lse.abs() * 2.0 ** -22).all()

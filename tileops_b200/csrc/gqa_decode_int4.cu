@@ -554,8 +554,9 @@ __global__ void __launch_bounds__(kAllThreads, Cfg<D, NT>::kBlocks) gqa_decode_i
           float top = abs_max<T, D / 8>(raw);
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-          // largest |n| in [2^13, 2^14), or [2^20, 2^21): below what the digits and the 22 bits of the sum hold
-          const int e = min(max((kDigits == 3 ? 20 : 13) + 127 - int(__float_as_uint(top) >> 23), -110), 110);
+          // largest |n| in [2^13, 2^14), or [2^20, 2^21): below what the digits and the 22 bits of the sum hold.  The largest
+          // finite bf16 asks for e = -114; a head whose largest |q| is below 2^-97 gets fewer bits than that.
+          const int e = min(max((kDigits == 3 ? 20 : 13) + 127 - int(__float_as_uint(top) >> 23), -114), 110);
           const float up = pow2f(e);
           // n = rint(q 2^e) as the low bits of 1.5 * 2^23 + n; with 128 (and 128 * 256) added its bytes are the signed
           // digits, of which the lower ones lie 128 too high
