@@ -479,7 +479,8 @@ int tb200_int4_cache_gather(const void* kv_pages, const int32_t* block_table, in
  *   lse [batch, heads] fp32 log2-domain or NULL; real_seqlen_kv [batch] int32 device
  *   block_table [batch, block_table_stride] int32, of which the first block_table_width columns are a row's
  * An empty sequence gives zeros (LSE -inf).  A page id outside [0, pool_pages), or a length beyond the table, makes that
- * sequence's o and lse NaN; nothing outside the pool and the table is read.
+ * sequence's o and lse NaN; nothing outside the pool and the table is read.  Scores are held in 32 bits: a head with an
+ * infinity or a NaN in q, or whose scores all lie below -1e30, gives NaN.
  * workspace: tb200_gqa_decode_int4_workspace_bytes() bytes, 256-byte aligned, the first
  * TB200_DECODE_INT4_ZERO_BYTES(batch, heads, heads_kv) zeroed once; as for tb200_gqa_decode it belongs to one shape
  * and one stream at a time.

@@ -412,3 +412,19 @@ def test_q_up_to_the_largest_bfloat16(H, D, top):
     to, tl = tolerances(q, pages, [300, 45], table, 16, sm_scale, 0.0)
     assert ((got.double().cpu() - ref).abs() <= to).all()
     assert ((lse.double().cpu() - ref_lse).abs() <= tl + ref_lse.abs() * 2.0 ** -22).all()
+
+
+@pytest.mark.parametrize("H,D", [(4, 128), (8, 64), (16, 128)])
+def test_scores_beyond_32_bits_do_not_pass_for_an_empty_sequence(H, D):
+    """Scores of -infinity throughout are no softmax: NaN, as in the plain form, and not the zeros of an empty sequence."""
+    page = 16
+    pages = torch.zeros(400, 1, F.int4_page_bytes(page, D), dtype=torch.uint8, device=DEV)
+    rows = torch.ones(400 * page, 1, D, dtype=torch.bfloat16, device=DEV)
+    F.int4_cache_append(rows, rows, torch.arange(400 * page, dtype=torch.int32, device=DEV), pages, page_size=page)
+    q = torch.full((4, H, D), -3e38, dtype=torch.bfloat16, device=DEV)
+    q[1] = 1.0
+    table = torch.arange(400, dtype=torch.int32, device=DEV).repeat(4, 1)
+    o, lse = F.gqa_decode_int4(q, pages, i32([1, 40, 0, 6400]), table, page_size=page, return_lse=True)
+    for b in (0, 3):
+        assert o[b].isnan().all() and lse[b].isnan().all()
+    assert (o[1] == 1).all() and (o[2] == 0).all() and (lse[2] == -float("inf")).all()

@@ -314,7 +314,8 @@ __device__ __forceinline__ void merge_add(Merged& a, float4 o, float4 ml) {
   a.M0 = m0;
   a.M1 = m1;
 }
-// Normalised result of a fragment to o and lse.  NaN passes on; a sum of 0 is an empty sequence.
+// Normalised result of a fragment to o and lse.  NaN passes on.  Sequences without a token own no tile and do not come here: a
+// sum of 0 means that every score was below kNegFloor (-infinity, where 32 bits do not hold it) and gives NaN.
 template <int D, typename TO>
 __device__ __forceinline__ void emit(const Int4DecodeParams& p, const Merged& a, int b, int head0, int n_heads, int frag,
                                      int lane) {
@@ -323,16 +324,16 @@ __device__ __forceinline__ void emit(const Int4DecodeParams& p, const Merged& a,
   const size_t row = size_t(b) * p.heads + head0 + h;
   TO* o = static_cast<TO*>(p.o) + row * D + d;
   if (h < n_heads) {
-    const float inv = a.L0 == 0.f ? 0.f : 1.f / a.L0;
+    const float inv = a.L0 == 0.f ? NAN : 1.f / a.L0;
     store_out<TO>(o, a.o.x * inv);
     store_out<TO>(o + 1, a.o.z * inv);
-    if (d == 0 && p.lse) p.lse[row] = a.L0 == 0.f ? -INFINITY : a.M0 + log2f(a.L0);
+    if (d == 0 && p.lse) p.lse[row] = a.L0 == 0.f ? NAN : a.M0 + log2f(a.L0);
   }
   if (h + 1 < n_heads) {
-    const float inv = a.L1 == 0.f ? 0.f : 1.f / a.L1;
+    const float inv = a.L1 == 0.f ? NAN : 1.f / a.L1;
     store_out<TO>(o + D, a.o.y * inv);
     store_out<TO>(o + D + 1, a.o.w * inv);
-    if (d == 0 && p.lse) p.lse[row + 1] = a.L1 == 0.f ? -INFINITY : a.M1 + log2f(a.L1);
+    if (d == 0 && p.lse) p.lse[row + 1] = a.L1 == 0.f ? NAN : a.M1 + log2f(a.L1);
   }
 }
 
