@@ -428,3 +428,36 @@ def test_scores_beyond_32_bits_do_not_pass_for_an_empty_sequence(H, D):
     for b in (0, 3):
         assert o[b].isnan().all() and lse[b].isnan().all()
     assert (o[1] == 1).all() and (o[2] == 0).all() and (lse[2] == -float("inf")).all()
+
+
+def chunk_problem(B, T, H=8, Hkv=2, D=128, page=16, W=2, pool=16, seed=0):
+    """A pool whose every token holds values, tables of distinct pages, and the rows of a chunk."""
+    g = torch.Generator().manual_seed(seed)
+    pages = torch.zeros(pool, Hkv, F.int4_page_bytes(page, D), dtype=torch.uint8, device=DEV)
+    rows = [torch.randn(pool * page, Hkv, D, generator=g).bfloat16().to(DEV) for _ in range(2)]
+    F.int4_cache_append(*rows, torch.arange(pool * page, dtype=torch.int32, device=DEV), pages, page_size=page)
+    table = torch.randperm(pool, generator=g)[:B * W].view(B, W).to(torch.int32).to(DEV)
+    q, k, v = (torch.randn(T, h, D, generator=g).bfloat16().to(DEV) for h in (H, Hkv, Hkv))
+    op = ops.GroupedQueryAttentionPrefillPagedInt4KVCacheFwdOp(B, H, Hkv, W, page, D)
+    op.validate_inputs = False
+    return op, q, k, v, pages, table
+
+
+def test_two_prefills_whose_launches_interleave(monkeypatch):
+    """Another call of the same shape on the same stream between this call's read-back and its attention, as a second host
+    thread can make it, must leave this call's keys and values alone."""
+    op, q, k, v, pages, table = chunk_problem(2, 9)
+    cu, old = i32([0, 4, 9]), i32([20, 9])
+    want = op(q, k, v, pages.clone(), cu, old, table, 5)
+    other = chunk_problem(2, 9, seed=1)
+    attend, inside = F.gqa_prefill_paged, []
+
+    def interleaved(*args, **kwargs):
+        if not inside:
+            inside.append(True)
+            other[0](*other[1:5], cu, old, other[5], 5)
+        return attend(*args, **kwargs)
+
+    monkeypatch.setattr(F, "gqa_prefill_paged", interleaved)
+    got = op(q, k, v, pages, cu, old, table, 5)
+    assert inside and torch.equal(got, want)

@@ -881,8 +881,8 @@ def gqa_prefill_paged_int4_cache(q: torch.Tensor, k_new: torch.Tensor, v_new: to
                                  sm_scale: Optional[float] = None, softcap: float = 0.0) -> torch.Tensor:
     """Packed prefill of one chunk per request over the 4-bit paged cache, appending the chunk: the cached tokens are read
     back as packed 16-bit K/V next to the chunk's own rows, the packed prefill runs on it, and the chunk is quantised into
-    the pages.  The packed buffer is sized by the capacity of the block table and kept per shape; nothing is read back from
-    the device."""
+    the pages.  The packed buffer is sized by the capacity of the block table (2 B W page_size Hkv D elements) and given
+    back to the allocator after the call; nothing is read back from the device."""
     _require_cuda(q=q, k_new=k_new, v_new=v_new, kv_pages=kv_pages)
     total_q, H, D = q.shape
     Hkv, B, device = k_new.shape[1], cu_seqlens_q.numel() - 1, q.device
@@ -893,13 +893,8 @@ def gqa_prefill_paged_int4_cache(q: torch.Tensor, k_new: torch.Tensor, v_new: to
     cu_kv[1:] = torch.cumsum(cache_seqlens + new_lens, 0)
     slots = paged_kv_plan(cache_seqlens, new_lens, block_table, None, None, total_q, page_size=page_size).slot_mapping
     total_kv = B * block_table.shape[1] * int(page_size)
-    key = (device, torch.cuda.current_stream(device).cuda_stream, "int4_cache_packed", total_kv, Hkv, D, q.dtype)
-    capturing = _capturing(device)
-    bufs = None if capturing else _WORKSPACES.get(key)
-    if bufs is None:
-        bufs = tuple(torch.empty((total_kv, Hkv, D), dtype=q.dtype, device=device) for _ in range(2))
-        if not capturing:
-            _WORKSPACES[key] = bufs
+    # The call's own: a buffer kept for the shape would be shared by two host threads whose launches interleave.
+    bufs = tuple(torch.empty((total_kv, Hkv, D), dtype=q.dtype, device=device) for _ in range(2))
     k_all, v_all = int4_cache_gather(kv_pages, block_table, cu_kv, total_kv, dim=D, page_size=page_size, dtype=q.dtype,
                                      cache_seqlens=cache_seqlens, cu_seqlens_new=cu_seqlens_q, k_new=k_new, v_new=v_new,
                                      out=bufs)
