@@ -461,3 +461,31 @@ def test_two_prefills_whose_launches_interleave(monkeypatch):
     monkeypatch.setattr(F, "gqa_prefill_paged", interleaved)
     got = op(q, k, v, pages, cu, old, table, 5)
     assert inside and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("cached", [33, 90, 2 ** 31 - 1, -1, -7, -2 ** 31])
+def test_prefill_of_a_request_longer_than_its_table_stays_with_that_request(cached):
+    """Lengths are range checked on the host; without that check a request that claims more tokens than its table has
+    becomes NaN, is not stored, and changes nothing for the others."""
+    op, q, k, v, pages, table = chunk_problem(3, 15)
+    cu = i32([0, 5, 9, 15])
+    before = pages.clone()
+    want = op(q, k, v, pages.clone(), cu, i32([10, 20, 20]), table, 6)
+    got = op(q, k, v, pages, cu, i32([10, cached, 20]), table, 6)
+    assert torch.equal(got[:5], want[:5]) and torch.equal(got[9:], want[9:])
+    assert got[5:9].isnan().all()
+    mine = table[1].long()
+    assert torch.equal(pages[mine], before[mine])
+
+
+def test_prefill_of_a_chunk_that_the_table_has_no_room_for():
+    """The attention of such a request is as well defined as any other; its chunk is not stored."""
+    op, q, k, v, pages, table = chunk_problem(3, 15, W=3)
+    narrow = ops.GroupedQueryAttentionPrefillPagedInt4KVCacheFwdOp(3, 8, 2, 2, 16, 128)
+    narrow.validate_inputs = False
+    cu, old = i32([0, 5, 9, 15]), i32([10, 30, 20])
+    before = pages.clone()
+    want = op(q, k, v, pages.clone(), cu, old, table, 6)
+    assert torch.equal(narrow(q, k, v, pages, cu, old, table[:, :2].contiguous(), 6), want)
+    mine = table[1].long()
+    assert torch.equal(pages[mine], before[mine])

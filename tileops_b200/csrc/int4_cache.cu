@@ -119,8 +119,11 @@ __global__ void __launch_bounds__(kThreads + 32, kBlocksPerSm) int4_gather_kerne
         if (p.cu[mid] <= g) lo = mid; else hi = mid - 1;
       }
       const int t = g - p.cu[lo];
-      if (p.cached && t >= p.cached[lo]) {
-        const long long from = (long long)p.cu_new[lo] + t - p.cached[lo];
+      const int cached = p.cached ? p.cached[lo] : 0x7fffffff;
+      if (cached < 0) {
+        src = -1;                           // no such length: NaN
+      } else if (p.cached && t >= cached) {
+        const long long from = (long long)p.cu_new[lo] + t - cached;
         src = from >= 0 && from < p.cu_new[p.batch] ? -3 - from : -1;     // a row that k_new does not have reads as NaN
       } else {
         const int column = t / p.page_size, off = t - column * p.page_size;

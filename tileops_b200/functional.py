@@ -773,7 +773,8 @@ def int4_cache_gather(kv_pages: torch.Tensor, block_table: torch.Tensor, cu_seql
     behind ``cu_seqlens_kv[-1]`` are left as they were (uninitialised in a new tensor).
 
     With ``cache_seqlens``, ``cu_seqlens_new``, ``k_new`` and ``v_new`` only the first ``cache_seqlens[b]`` rows of a request
-    come from the cache and the rest from rows ``cu_seqlens_new[b] ..`` of ``k_new`` / ``v_new``."""
+    come from the cache and the rest from rows ``cu_seqlens_new[b] ..`` of ``k_new`` / ``v_new``, which have
+    ``cu_seqlens_new[-1]`` rows; a negative ``cache_seqlens[b]`` makes the request NaN."""
     _require_cuda(kv_pages=kv_pages)
     if kv_pages.dim() != 3:
         raise ValueError(f"kv_pages must be [pages, heads_kv, page bytes], got {tuple(kv_pages.shape)}")
@@ -881,18 +882,22 @@ def gqa_prefill_paged_int4_cache(q: torch.Tensor, k_new: torch.Tensor, v_new: to
                                  sm_scale: Optional[float] = None, softcap: float = 0.0) -> torch.Tensor:
     """Packed prefill of one chunk per request over the 4-bit paged cache, appending the chunk: the cached tokens are read
     back as packed 16-bit K/V next to the chunk's own rows, the packed prefill runs on it, and the chunk is quantised into
-    the pages.  The packed buffer is sized by the capacity of the block table (2 B W page_size Hkv D elements) and given
-    back to the allocator after the call; nothing is read back from the device."""
+    the pages.  The packed buffer is sized by the capacity of the block table (K and V of B W page_size + T tokens) and
+    given back to the allocator after the call; nothing is read back from the device.  ``cache_seqlens[b]`` outside what
+    the table holds makes request b NaN; a chunk that the table has no room for is attended to but not stored."""
     _require_cuda(q=q, k_new=k_new, v_new=v_new, kv_pages=kv_pages)
     total_q, H, D = q.shape
     Hkv, B, device = k_new.shape[1], cu_seqlens_q.numel() - 1, q.device
     if total_q == 0:
         return torch.empty_like(q)
     new_lens = cu_seqlens_q[1:] - cu_seqlens_q[:-1]
+    # A request that claims more tokens than its table has (or fewer than none) gets rows of its own that read as NaN: none
+    # of the others' move out of the buffer.
+    capacity = block_table.shape[1] * int(page_size)
     cu_kv = torch.zeros(B + 1, dtype=torch.int32, device=device)
-    cu_kv[1:] = torch.cumsum(cache_seqlens + new_lens, 0)
+    cu_kv[1:] = torch.cumsum(cache_seqlens.clamp(0, capacity) + new_lens, 0)
     slots = paged_kv_plan(cache_seqlens, new_lens, block_table, None, None, total_q, page_size=page_size).slot_mapping
-    total_kv = B * block_table.shape[1] * int(page_size)
+    total_kv = B * capacity + total_q
     # The call's own: a buffer kept for the shape would be shared by two host threads whose launches interleave.
     bufs = tuple(torch.empty((total_kv, Hkv, D), dtype=q.dtype, device=device) for _ in range(2))
     k_all, v_all = int4_cache_gather(kv_pages, block_table, cu_kv, total_kv, dim=D, page_size=page_size, dtype=q.dtype,
