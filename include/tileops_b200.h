@@ -459,10 +459,10 @@ int tb200_qk_norm_rope(const void* q, const void* k, const void* v, void* q_out,
  *
  * gather reads it back: output rows cu_seqlens_kv[b] .. cu_seqlens_kv[b + 1] are request b's tokens 0, 1, ..: all of
  * them from the cache (cache_seqlens NULL), or the first cache_seqlens[b] from the cache and the rest from rows
- * cu_seqlens_new[b] .. of k_new / v_new.  scale * code + offset in fp32, rounded to dtype.  total_tokens bounds the rows
- * (rows at or behind cu_seqlens_kv[batch] are left as they were); a page id outside the pool reads as NaN, and so does a
- * row outside 0 .. cu_seqlens_new[batch] - 1, which is the number of rows of k_new and v_new; so does all of a request with
- * a negative cache_seqlens[b].
+ * cu_seqlens_new[b] .. of k_new / v_new.  scale * code + offset in fp32, rounded to dtype (F16: saturated at +-65504).
+ * total_tokens bounds the rows (rows at or behind cu_seqlens_kv[batch] are left as they were); a page id outside the pool
+ * reads as NaN, and so does a row outside 0 .. cu_seqlens_new[batch] - 1, which is the number of rows of k_new and v_new; so
+ * does all of a request with a negative cache_seqlens[b].
  * ------------------------------------------------------------------------- */
 int tb200_int4_cache_append(const void* k, const void* v, const int32_t* slots, void* kv_pages, int dtype, int tokens,
                             int heads_kv, int dim, int page_size, int64_t pool_tokens, int64_t k_token_stride,

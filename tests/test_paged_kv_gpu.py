@@ -475,3 +475,21 @@ def test_a_slot_of_a_page_that_32_bits_do_not_hold_is_none(bad, page):
     # the same from the stack
     plan = ops.PagedKVCachePlanFwdOp(1, 2, page)(i32([page]), i32([2]), i32([[1, 0]]), i32([4, bad]), i32([2]), 2)
     assert plan.slot_mapping.tolist() == ([bad * page, bad * page + 1] if fits else [-1, -1])
+
+
+# ---- values at the ends of the quantiser's range ------------------------------------------------------------------------
+@pytest.mark.parametrize("D", [64, 128])
+def test_float16_read_back_saturates(D):
+    """15 steps of f16((65504 + 65504) / 15) = 8736 end 32 beyond the largest float16: the read-back must not overflow."""
+    page, Hkv = 16, 1
+    big = torch.finfo(torch.float16).max
+    k = torch.zeros(4, Hkv, D, dtype=torch.float16)
+    k[:, :, ::2], k[:, :, 1::2] = big, -big
+    k[2:, 0, 3] = float("inf")
+    v = -k
+    v[3, 0, 5] = float("nan")
+    pages = torch.zeros(1, Hkv, F.int4_page_bytes(page, D), dtype=torch.uint8, device=DEV)
+    ops.Int4KVCacheAppendFwdOp(Hkv, D, page)(k.to(DEV), v.to(DEV), i32([0, 1, 2, 3]), pages)
+    got_k, got_v = ops.Int4KVCacheGatherFwdOp(Hkv, D, page, torch.float16)(pages, i32([[0]]), i32([0, 4]), 4)
+    assert torch.equal(got_k.cpu(), torch.nan_to_num(k, posinf=big))
+    assert torch.equal(got_v[:3].cpu(), torch.nan_to_num(v[:3], neginf=-big)) and got_v[3].isnan().all()

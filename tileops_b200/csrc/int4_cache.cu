@@ -1,6 +1,6 @@
 // Reads a 4-bit paged KV cache back as packed 16-bit K and V, sm_100a: the cache side of a chunked prefill, whose
 // tcgen05 attention kernel takes 16-bit operands.  value = scale * code + offset in fp32 (the product is exact), rounded
-// once.  HBM bound: dim + 8 bytes read and 4 dim written per token and KV head.
+// once (float16: saturated at +-65504).  HBM bound: dim + 8 bytes read and 4 dim written per token and KV head.
 #include "int4_cache.cuh"
 
 namespace tb200 {
@@ -30,6 +30,15 @@ struct GatherParams {
 constexpr int kTokens = 8;
 constexpr int kAhead = 4;
 constexpr int kBlocksPerSm = 5;
+
+// Two values side by side.  15 steps between +-65504 end 32 beyond the largest float16 (their scale is rounded to 8736): a
+// float16 read-back saturates, as the append does.  bfloat16 holds them.
+template <typename T>
+__device__ __forceinline__ uint32_t pack_value(float a, float b) {
+  const uint32_t v = pack2<T>(a, b);
+  if constexpr (std::is_same<T, __half>::value) return max2_nan<T>(min2_nan<T>(v, 0x7bff7bffu), 0xfbfffbffu);
+  return v;
+}
 
 // The rows of one piece, by the kThreads working threads.
 template <typename T, int D>
@@ -91,7 +100,8 @@ __device__ __forceinline__ void expand(const GatherParams& p, int g0, const long
           x[2 * b + 4] = fmaf(lo, even.y, m);
           x[2 * b + 5] = fmaf(hi, odd.y, m);
         }
-        out[i * (D / 16)] = make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
+        out[i * (D / 16)] = make_uint4(pack_value<T>(x[0], x[1]), pack_value<T>(x[2], x[3]), pack_value<T>(x[4], x[5]),
+                                       pack_value<T>(x[6], x[7]));
       }
     }
   }

@@ -247,7 +247,7 @@ class Int4KVCacheGatherFwdOp(Op):
     """Reads a 4-bit cache back: ``forward(kv_pages, block_table, cu_seqlens_kv, total_tokens)`` returns K and V
     ``[total_tokens,Hkv,D]`` in ``dtype``; rows ``cu_seqlens_kv[b] .. cu_seqlens_kv[b + 1]`` are request b's tokens from 0 on.
     ``total_tokens`` may be an upper bound (rows behind the last request's are left uninitialised).  A page id outside the
-    pool reads as NaN."""
+    pool reads as NaN; float16 values saturate at +-65504."""
 
     def __init__(self, heads_kv: int, dim: int, page_size: int, dtype: torch.dtype = torch.bfloat16,
                  kernel_map: Optional[Dict[str, type]] = None) -> None:
