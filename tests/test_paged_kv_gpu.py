@@ -493,3 +493,21 @@ def test_float16_read_back_saturates(D):
     got_k, got_v = ops.Int4KVCacheGatherFwdOp(Hkv, D, page, torch.float16)(pages, i32([[0]]), i32([0, 4]), 4)
     assert torch.equal(got_k.cpu(), torch.nan_to_num(k, posinf=big))
     assert torch.equal(got_v[:3].cpu(), torch.nan_to_num(v[:3], neginf=-big)) and got_v[3].isnan().all()
+
+
+def test_rows_whose_step_is_a_subnormal_keep_the_stated_bound():
+    """Half a step, 15 times the rounding of the scale and the rounding of the offset and of the read-back, each 2^-11 of the
+    value or 2^-25, half of float16's smallest subnormal; a step of 2^-25 or less has scale 0 and is all rounding."""
+    T, D, page = 32, 64, 16
+    g = torch.Generator().manual_seed(6)
+    span = torch.logspace(-8, -3, T, dtype=torch.float64)[:, None, None]
+    x = (torch.rand(T, 1, D, generator=g, dtype=torch.float64) * span).to(torch.float16)
+    pages = torch.zeros(T // page, 1, F.int4_page_bytes(page, D), dtype=torch.uint8, device=DEV)
+    ops.Int4KVCacheAppendFwdOp(1, D, page)(x.to(DEV), -x.to(DEV), i32(list(range(T))), pages)
+    k, v = ops.Int4KVCacheGatherFwdOp(1, D, page, torch.float16)(pages, i32([[0, 1]]), i32([0, T]), T)
+    x = x.double()
+    step = (x.amax(-1, keepdim=True) - x.amin(-1, keepdim=True)) / 15
+    rounding = lambda y: torch.clamp(y.abs() * 2 ** -11, min=2 ** -25)  # noqa: E731
+    tol = step / 2 + 15 * rounding(step) + rounding(x.amax(-1, keepdim=True)) + rounding(x.abs() + step)
+    assert_within(k, x, tol, "k")
+    assert_within(v, -x, tol, "v")

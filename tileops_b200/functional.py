@@ -745,8 +745,8 @@ def int4_cache_append(k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tens
                       page_size: int) -> None:
     """Quantises k and v ``[T,Hkv,D]`` into the rows ``slot_mapping`` (int32 ``[T]``) of the 4-bit pool, in place: 15
     steps between a row's smallest and largest value, one float16 scale and offset per token and KV head (error at most
-    half a step plus the rounding of the scale, 15 x 2^-11 of a step).  Rows outside the pool are skipped; rows of one call
-    must be distinct."""
+    half a step, 15 times the rounding of the scale - 2^-11 of a step, or 2^-25 below float16's normal numbers - and the
+    rounding of the offset).  Rows outside the pool are skipped; rows of one call must be distinct."""
     _require_cuda(k=k)
     _check_kv_rows(k, v)
     device, dtype = k.device, k.dtype

@@ -217,8 +217,9 @@ class Int4KVCacheAppendFwdOp(Op):
     ``kv_pages`` is uint8 ``[pages, Hkv, page_size * (D + 8)]`` (:meth:`page_bytes`), modified in place; the library's header
     gives its layout and :func:`tileops_b200.functional.int4_cache_views` its parts.  Each row (one token of one KV head)
     has 15 equal steps between its smallest and largest value and a float16 scale and offset; value = scale * code +
-    offset is off by at most half a step and 15 x 2^-11 of one (the scale's rounding).  Values beyond +-65504 saturate; a
-    row with a NaN reads as NaN.  ``slot_mapping``: int32 ``[T]``, distinct, rows outside the pool are skipped."""
+    offset is off by at most half a step and 15 times the rounding of the scale (2^-11 of a step, or 2^-25 where the step is
+    below 2^-14, float16's smallest normal number), and by the offset's rounding where it is no float16.  Values beyond +-65504
+    saturate; a row with a NaN reads as NaN.  ``slot_mapping``: int32 ``[T]``, distinct, rows outside the pool are skipped."""
 
     def __init__(self, heads_kv: int, dim: int, page_size: int, kernel_map: Optional[Dict[str, type]] = None) -> None:
         _validate_positive(heads_kv=heads_kv)
