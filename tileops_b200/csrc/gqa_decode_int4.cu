@@ -108,6 +108,7 @@ struct Cfg {
   static_assert(kSegmentCost < kMinRun, "no range lies in a gap");
   static_assert(2 * kBlocks <= kSlotsPerSm, "every range has its slots");
   static_assert(qslots % 128 == 0 && dump % 16 == 0 && bars % 8 == 0, "layout");
+  static_assert(plan + (2 * kMaxBatch + 1) * 4 <= 227 * 1024, "the largest batch fits a block");
 };
 
 template <int D, int NT>
@@ -968,14 +969,17 @@ template <int D, int NT, bool kPair, typename T, typename TO>
 int launch(const Int4DecodeParams& p, cudaStream_t stream) {
   auto kern = gqa_decode_int4_kernel<D, NT, kPair, T, TO>;
   const size_t smem = smem_bytes<D, NT>(p.batch);
-  static thread_local size_t configured[64] = {0}, sized_for[64] = {0};
+  static thread_local bool configured[64] = {false};
+  static thread_local size_t sized_for[64] = {0};
   static thread_local int resident[64] = {0};
   int dev = 0;
   TB200_CUDA_CHECK(cudaGetDevice(&dev));
   if (dev < 0 || dev >= 64) TB200_FAIL(TB200_ERR_UNSUPPORTED, "device index %d", dev);
-  if (configured[dev] < smem) {
-    TB200_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
-    configured[dev] = smem;
+  if (!configured[dev]) {
+    // The limit belongs to the function, not to this thread: every thread sets the one that the largest batch needs, so
+    // that none takes it from another.
+    TB200_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem_bytes<D, NT>(kMaxBatch))));
+    configured[dev] = true;
   }
   if (sized_for[dev] != smem) {
     int n = 0;
