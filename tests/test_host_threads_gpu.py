@@ -1,6 +1,7 @@
 """Launches of one kernel from several host threads with problems of different size: what one thread's call sets up for a
 kernel must not take anything from another thread's."""
 
+import threading
 from concurrent.futures import ThreadPoolExecutor
 
 import pytest
@@ -33,3 +34,29 @@ def test_int4_decode_of_a_large_and_of_a_small_batch(H, D):
         return lambda: F.gqa_decode_int4(q, pages, lens, table, page_size=16)
 
     alternate(call(900), call(3))
+
+
+def test_plan_and_release_of_batches_above_48_kilobytes():
+    """The large and the small batch both ask for more shared memory than a function has by itself; two threads launch them
+    at the same time."""
+    page, rounds, start = 16, 1000, threading.Barrier(2, timeout=60)
+
+    def prepare(batch):
+        seq = torch.arange(batch, dtype=torch.int32, device=DEV) % 40
+        new, table = torch.ones_like(seq), torch.arange(batch * 3, dtype=torch.int32, device=DEV).view(batch, 3)
+        done, free, count = (torch.zeros(n, dtype=t, device=DEV) for n, t in ((batch, torch.bool), (4, torch.int32), (1, torch.int32)))
+
+        def run():
+            start.wait()
+            for _ in range(rounds):
+                got = F.paged_kv_plan(seq, new, table, None, None, batch, page_size=page)
+                F.paged_kv_release(done, seq, table, free, count, page_size=page)
+            want = F.paged_kv_plan(seq, new, table, None, None, batch, page_size=page)
+            return all(torch.equal(a, b) for a, b in zip(got, want) if a is not None)
+
+        return run
+
+    calls = [prepare(batch) for batch in (4096, 3200)]
+    with ThreadPoolExecutor(2) as pool:
+        results = [pool.submit(call) for call in calls]
+        assert all(r.result(timeout=120) for r in results)

@@ -254,6 +254,16 @@ int plan_threads(int batch, int total) {
   return want <= 128 ? 128 : want <= 256 ? 256 : want <= 512 ? 512 : kPlanThreads;
 }
 
+// More shared memory than a function has by itself.  The limit belongs to the function and not to this thread: every thread
+// sets the one that the largest batch needs, so that none takes it from another between its own setting and its launch.
+int allow_largest_batch(size_t smem) {
+  if (smem <= 48 * 1024) return TB200_OK;
+  const int most = int(plan_smem(kMaxRequests));
+  TB200_CUDA_CHECK(cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+  TB200_CUDA_CHECK(cudaFuncSetAttribute(paged_release_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+  return TB200_OK;
+}
+
 int check_plan_sizes(int batch, int width, int page, int64_t capacity) {
   if (batch <= 0 || width <= 0 || page <= 0) TB200_FAIL(TB200_ERR_BAD_ARGUMENT, "batch, pages per request and page_size must be positive");
   if (batch > kMaxRequests) TB200_FAIL(TB200_ERR_UNSUPPORTED, "at most %d requests, got %d", kMaxRequests, batch);
@@ -303,8 +313,7 @@ extern "C" int tb200_paged_kv_plan(const int32_t* seq_lens, const int32_t* new_l
   attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  if (cfg.dynamicSmemBytes > 48 * 1024)
-    TB200_CUDA_CHECK(cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(cfg.dynamicSmemBytes)));
+  if (const int st = allow_largest_batch(cfg.dynamicSmemBytes)) return st;
   TB200_CUDA_CHECK(cudaLaunchKernelEx(&cfg, paged_plan_kernel, p));
   return TB200_OK;
 }
@@ -316,8 +325,7 @@ extern "C" int tb200_paged_kv_release(const uint8_t* finished, int32_t* seq_lens
   if (!finished || !seq_lens || !block_table || !free_count || (free_capacity > 0 && !free_pages))
     TB200_FAIL(TB200_ERR_BAD_ARGUMENT, "pointers must be non-null");
   const size_t smem = plan_smem(batch);
-  if (smem > 48 * 1024)
-    TB200_CUDA_CHECK(cudaFuncSetAttribute(paged_release_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
+  if (const int st = allow_largest_batch(smem)) return st;
   paged_release_kernel<<<1, plan_threads(batch, 0), smem, static_cast<cudaStream_t>(stream)>>>(
       finished, seq_lens, block_table, block_table_stride, free_pages, free_count, int(free_capacity), batch,
       max_pages_per_req, page_size);
