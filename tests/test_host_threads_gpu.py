@@ -60,3 +60,23 @@ def test_plan_and_release_of_batches_above_48_kilobytes():
     with ThreadPoolExecutor(2) as pool:
         results = [pool.submit(call) for call in calls]
         assert all(r.result(timeout=120) for r in results)
+
+
+def decode_call(batch, fp8, config):
+    inp = W.make_paged_decode(5, 2, 8, 2, 128, 64, lens=[20, 64], device=DEV, dtype=torch.bfloat16)
+    q = inp.q[:1].repeat(batch, 1, 1)
+    lens = torch.full((batch,), 20, dtype=torch.int32, device=DEV)
+    table = inp.block_table[:1].repeat(batch, 1)
+    k, v, scales = inp.k, inp.v, {}
+    if fp8:
+        k, v = k.to(torch.float8_e4m3fn), v.to(torch.float8_e4m3fn)
+        ones = torch.ones(k.shape[0] // 64, 2, device=DEV)
+        scales = dict(k_scale=ones, v_scale=ones)
+    return lambda: F.gqa_decode(q, k, v, real_seqlen_kv=lens, block_table=table, page_size=64, config=config, **scales)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_tma_decode_of_a_large_and_of_a_small_batch(fp8):
+    alternate(decode_call(300, fp8, None), decode_call(3, fp8, None))
+    decode_call(3, fp8, None)()
+    assert F.decode_last_kernel() == "tma"

@@ -843,16 +843,19 @@ template <int D, bool FP8, typename T, typename TO>
 int launch_tma(const CUtensorMap& mk, const CUtensorMap& mv, const DecodeParams& p, cudaStream_t stream) {
   auto kern = gqa_decode_tma_kernel<D, FP8, T, TO>;
   const size_t smem = tma_smem_bytes<D, FP8>(p.batch);
-  static thread_local size_t configured[64] = {0};
+  static thread_local bool configured[64] = {false};
   static thread_local size_t sized_for[64] = {0};
   static thread_local int resident[64] = {0};
   int dev = 0;
   TB200_CUDA_CHECK(cudaGetDevice(&dev));
   if (dev < 0 || dev >= 64) return kTmaNotApplicable;
-  if (smem > 227 * 1024) return kTmaNotApplicable;
-  if (configured[dev] < smem) {
-    TB200_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    configured[dev] = smem;
+  if (!configured[dev]) {
+    // The limit belongs to the function, not to this thread: every thread sets the one that the largest batch needs, so
+    // that none takes it from another.
+    static_assert(TmaCfg<D, FP8>::plan + (2 * kMaxBatch + 1) * 4 + 1024 <= 227 * 1024, "the largest batch fits a CTA");
+    TB200_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                          (int)tma_smem_bytes<D, FP8>(kMaxBatch)));
+    configured[dev] = true;
   }
   if (sized_for[dev] != smem) {
     int n = 0;
