@@ -80,3 +80,10 @@ def test_tma_decode_of_a_large_and_of_a_small_batch(fp8):
     alternate(decode_call(300, fp8, None), decode_call(3, fp8, None))
     decode_call(3, fp8, None)()
     assert F.decode_last_kernel() == "tma"
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_cp_async_decode_of_a_large_and_of_a_small_batch(fp8):
+    alternate(decode_call(300, fp8, {"tma": False}), decode_call(3, fp8, {"tma": False}))
+    decode_call(3, fp8, {"tma": False})()
+    assert F.decode_last_kernel() == "cp_async"

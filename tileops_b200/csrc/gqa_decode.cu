@@ -80,6 +80,7 @@ size_t smem_bytes(int batch, int nt) {
   size_t ring = size_t(C::kStages) * C::kStageBytes;
   size_t merge = size_t(kWarps) * (8 * nt) * (C::kOStride + 2) * 4;
   size_t a = ring > merge ? ring : merge;
+  static_assert(C::kStages * C::kStageBytes + (2 * kMaxBatch + 1) * 4 + 128 <= 227 * 1024, "the largest batch fits a CTA");
   return a + size_t(2 * batch + 1) * 4 + 128;   // run-count prefix [batch + 1] and the lengths [batch]
 }
 
@@ -751,18 +752,21 @@ template <int D, bool FP8, typename T, int NT, typename TO, bool F8M = false, bo
 int launch(const DecodeParams& p, cudaStream_t stream) {
   auto kern = gqa_decode_kernel<D, FP8, T, NT, TO, F8M, WIDE>;
   const size_t smem = smem_bytes<D, FP8, WIDE>(p.batch, NT);
-  // per device: the largest dynamic shared memory size configured so far, and the number of CTAs an
-  // SM holds at the size of the last launch (the grid is one CTA per resident slot: a CTA that starts
-  // late finds the item queue empty and only costs its plan)
-  static thread_local size_t configured[64] = {0};
+  // per device: whether the limit below is set, and the number of CTAs an SM holds at the size of the
+  // last launch (the grid is one CTA per resident slot: a CTA that starts late finds the item queue empty
+  // and only costs its plan)
+  static thread_local bool configured[64] = {false};
   static thread_local size_t sized_for[64] = {0};
   static thread_local int resident[64] = {0};
   int dev = 0;
   TB200_CUDA_CHECK(cudaGetDevice(&dev));
   if (dev < 0 || dev >= 64) TB200_FAIL(TB200_ERR_UNSUPPORTED, "device index %d is outside [0, 64)", dev);
-  if (configured[dev] < smem) {
-    TB200_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    configured[dev] = smem;
+  if (!configured[dev]) {
+    // The limit belongs to the function, not to this thread: every thread sets the one that the largest
+    // batch needs, so that none takes it from another.
+    TB200_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                          (int)smem_bytes<D, FP8, WIDE>(kMaxBatch, NT)));
+    configured[dev] = true;
   }
   if (sized_for[dev] != smem) {
     int n = 0;
