@@ -104,6 +104,8 @@ int tb200_version(void);
 #define TB200_DECODE_NO_TMA 8    /* keep the cp.async kernel where the TMA kernel would apply */
 #define TB200_DECODE_CHUNK_TILES_SHIFT 8 /* bits 8..23: fixed split-KV run length in 64-token tiles (0 = cost model) */
 #define TB200_DECODE_CHUNK_TILES(n) (((n) & 0xFFFF) << TB200_DECODE_CHUNK_TILES_SHIFT)
+#define TB200_DECODE_WAIT_LOG2_SHIFT 24  /* bits 24..28, tb200_gqa_decode_int4: limit of a device-side wait, 2^n clock ticks
+                                            (0 = about half a second) */
 
 size_t tb200_gqa_decode_workspace_bytes(int batch, int heads, int heads_kv, int dim);
 
@@ -484,7 +486,8 @@ int tb200_int4_cache_gather(const void* kv_pages, const int32_t* block_table, in
  * infinity or a NaN in q, or whose scores all lie below -1e30, gives NaN.
  * workspace: tb200_gqa_decode_int4_workspace_bytes() bytes, 256-byte aligned, the first
  * TB200_DECODE_INT4_ZERO_BYTES(batch, heads, heads_kv) zeroed once; as for tb200_gqa_decode it belongs to one shape
- * and one stream at a time.
+ * and one stream at a time, its status word is the int32 at byte 8, and after a wait that ran out (601, 602, 603) o and lse
+ * are partly unwritten and the workspace must be zeroed again.
  * ------------------------------------------------------------------------- */
 #define TB200_DECODE_INT4_ZERO_BYTES(batch, heads, heads_kv) (((size_t)(batch) * (size_t)(heads) + 8) * 4)
 size_t tb200_gqa_decode_int4_workspace_bytes(int batch, int heads, int heads_kv, int dim);

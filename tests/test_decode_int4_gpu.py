@@ -489,3 +489,17 @@ def test_prefill_of_a_chunk_that_the_table_has_no_room_for():
     assert torch.equal(narrow(q, k, v, pages, cu, old, table[:, :2].contiguous(), 6), want)
     mine = table[1].long()
     assert torch.equal(pages[mine], before[mine])
+
+
+def test_a_wait_that_runs_out_ends_the_launch_and_is_reported():
+    """A limit far below a copy's latency: the launch gives up, says so, and the next call is as good as ever."""
+    q, pages, lens, table = make([60000, 3000, 500], 32, 8, 128, 16, seed=21)
+    want = F.gqa_decode_int4(q, pages, lens, table, page_size=16)
+    assert F.decode_status() == 0
+    for _ in range(3):
+        F.gqa_decode_int4(q, pages, lens, table, page_size=16, config={"wait_log2": 1})
+        torch.cuda.synchronize()
+        assert F.decode_status() in (601, 602, 603)
+        assert F.decode_status() == 0
+        assert torch.equal(F.gqa_decode_int4(q, pages, lens, table, page_size=16), want)
+    assert F.decode_status() == 0

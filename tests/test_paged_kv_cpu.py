@@ -241,3 +241,10 @@ def test_oracle_cache_round_trip_and_views():
 def test_oracle_plan_by_hand():
     got = O.plan_ref([15, 32], [2, 1], [[4, 0], [5, 6]], [7, 8, 9], 3, 4, 16)
     assert got == ([[4, 9], [5, 6]], [0, 2, 3], [4 * 16 + 15, 9 * 16, -1, -1], [15, 16, 32, 0], [17, 32], 2, [1, 0])
+
+
+def test_decode_flags_of_the_wait_limit():
+    assert _native.decode_flags({"wait_log2": 5, "chunk_tiles": 3}) == (5 << 24) | (3 << 8)
+    for bad in (-1, 32):
+        with pytest.raises(ValueError, match="wait_log2"):
+            _native.decode_flags({"wait_log2": bad})

@@ -25,6 +25,7 @@ F16, BF16, E4M3, F32 = 0, 1, 2, 3
 # variant flags of tb200_gqa_decode (TB200_DECODE_* in include/tileops_b200.h)
 DECODE_WIDE_ON, DECODE_WIDE_OFF, DECODE_FP8_MMA, DECODE_NO_TMA = 1, 2, 4, 8
 DECODE_CHUNK_TILES_SHIFT = 8
+DECODE_WAIT_LOG2_SHIFT = 24
 # kinds of cache of tb200_qk_norm_rope (TB200_CACHE_* in include/tileops_b200.h)
 CACHE_NONE, CACHE_16BIT, CACHE_INT4 = 0, 1, 2
 PREFILL_TWO_TILES = 1
@@ -41,7 +42,8 @@ def prefill_flags(config: "dict | None") -> int:
 def decode_flags(config: "dict | None") -> int:
     """Variant flags from a kernel ``config`` dict: ``wide`` (True / False / absent = the library's
     choice), ``fp8_mma``, ``tma`` (False keeps the cp.async kernel), ``chunk_tiles`` (fixed split-KV
-    run length in 64-token tiles)."""
+    run length in 64-token tiles), ``wait_log2`` (4-bit cache: a device-side wait gives up after 2^n
+    clock ticks instead of about half a second)."""
     if not config:
         return 0
     flags = 0
@@ -55,7 +57,10 @@ def decode_flags(config: "dict | None") -> int:
     chunk = int(config.get("chunk_tiles") or 0)
     if not 0 <= chunk <= 0xFFFF:
         raise ValueError(f"chunk_tiles={chunk} is outside [0, 65535]")
-    return flags | (chunk << DECODE_CHUNK_TILES_SHIFT)
+    wait = int(config.get("wait_log2") or 0)
+    if not 0 <= wait <= 31:
+        raise ValueError(f"wait_log2={wait} is outside [0, 31]")
+    return flags | (chunk << DECODE_CHUNK_TILES_SHIFT) | (wait << DECODE_WAIT_LOG2_SHIFT)
 
 _DTYPE_CODE = {torch.float16: F16, torch.bfloat16: BF16, torch.float32: F32}
 if hasattr(torch, "float8_e4m3fn"):

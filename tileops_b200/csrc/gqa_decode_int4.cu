@@ -262,6 +262,13 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
   if (mbar_try_wait(bar, parity)) return true;
   return mbar_wait_slow(bar, parity, abort_flag, status, code, limit, sleep);
 }
+// The same by a whole warp, whose lanes get one answer: where one of them gives up, none goes on to a shuffle or a vote that
+// it no longer takes part in.
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code,
+                                               long long limit) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  return __all_sync(0xffffffffu, mbar_wait_slow(bar, parity, abort_flag, status, code, limit, 0));
+}
 
 template <int kWords>
 __device__ __forceinline__ void lds_words(uint32_t (&w)[kWords], const unsigned char* at) {
@@ -516,12 +523,12 @@ __global__ void __launch_bounds__(kAllThreads, Cfg<D, NT>::kBlocks) gqa_decode_i
     // thread's own stores only.
     uint32_t dump_par = 0, merged_par = 1;     // the dump area starts out free
     auto wait_dump = [&]() -> bool {
-      if (!mbar_wait(bar_dump, dump_par, s_abort, status, 603, limit)) { alive = false; return false; }
+      if (!mbar_wait_warp(bar_dump, dump_par, s_abort, status, 603, limit)) { alive = false; return false; }
       dump_par ^= 1;
       return true;
     };
     auto wait_merged = [&]() -> bool {
-      if (!mbar_wait(bar_merged, merged_par, s_abort, status, 603, limit)) { alive = false; return false; }
+      if (!mbar_wait_warp(bar_merged, merged_par, s_abort, status, 603, limit)) { alive = false; return false; }
       merged_par ^= 1;
       return true;
     };
@@ -534,7 +541,7 @@ __global__ void __launch_bounds__(kAllThreads, Cfg<D, NT>::kBlocks) gqa_decode_i
       for (unsigned u = range_begin; alive && u < range_end; ++round) {
         const int slot = round & 1;
         const bool first = u == range_begin;
-        if (!mbar_wait(bar_item_full(slot), (round >> 1) & 1, s_abort, status, 602, limit)) { alive = false; break; }
+        if (!mbar_wait_warp(bar_item_full(slot), (round >> 1) & 1, s_abort, status, 602, limit)) { alive = false; break; }
         const Segment& d = *reinterpret_cast<const Segment*>(smem + C::segs + slot * 64);
         u = d.next;
         const int n_heads = min(p.hb, p.group - d.hbi * p.hb), tile0 = d.tile0, tile1 = d.tile1, len = d.len;
@@ -632,7 +639,7 @@ __global__ void __launch_bounds__(kAllThreads, Cfg<D, NT>::kBlocks) gqa_decode_i
         }
 
         for (int tile = tile0; tile < tile1; ++tile) {
-          if (!mbar_wait(bar_full(stage), stage_par, s_abort, status, 602, limit)) { alive = false; break; }
+          if (!mbar_wait_warp(bar_full(stage), stage_par, s_abort, status, 602, limit)) { alive = false; break; }
           const unsigned char* st = smem + C::ring + stage * C::kStageBytes + warp * C::kRec;
           const int tok0 = (tile * C::kRecords + warp) * kInt4Tokens + my_tau;
 
@@ -1054,7 +1061,8 @@ extern "C" int tb200_gqa_decode_int4(const void* q, const void* kv_pages, void* 
   p.counters = static_cast<int*>(workspace);
   p.part_o = reinterpret_cast<float4*>(static_cast<unsigned char*>(workspace) + L.counters_bytes);
   p.part_ml = reinterpret_cast<float4*>(static_cast<unsigned char*>(workspace) + L.counters_bytes + L.part_o_bytes);
-  p.wait_cycles = 1000000000LL;   // about 0.5 s
+  const int wait_log2 = (flags >> TB200_DECODE_WAIT_LOG2_SHIFT) & 31;
+  p.wait_cycles = wait_log2 ? 1LL << wait_log2 : 1000000000LL;   // about 0.5 s
   static_assert(Cfg<128, 1>::kRecords == 8 && Cfg<128, 2>::kRecords == 8 && Cfg<64, 1>::kRecords == 8 && Cfg<64, 2>::kRecords == 8,
                 "the copies' sizes");
   p.records_per_copy = 1;
