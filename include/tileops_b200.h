@@ -492,6 +492,11 @@ int tb200_int4_cache_gather(const void* kv_pages, const int32_t* block_table, in
 #define TB200_DECODE_INT4_ZERO_BYTES(batch, heads, heads_kv) (((size_t)(batch) * (size_t)(heads) + 8) * 4)
 size_t tb200_gqa_decode_int4_workspace_bytes(int batch, int heads, int heads_kv, int dim);
 
+/* *code (host memory): 0, or the code of a wait of any tb200_gqa_decode_int4 launch on the current device that ran out since
+ * the word was last cleared, whatever became of its workspace (a CUDA graph that zeroes it on every replay).  Synchronises with
+ * `stream`; launches on other streams have to be waited for first.  reset: clear the word after a non-zero read. */
+int tb200_gqa_decode_int4_status(int32_t* code, int reset, void* stream);
+
 int tb200_gqa_decode_int4(const void* q, const void* kv_pages, void* o, float* lse, const int32_t* real_seqlen_kv,
                           const int32_t* block_table, int64_t block_table_stride, int block_table_width, int q_dtype,
                           int o_dtype, int batch, int heads, int heads_kv, int dim, int page_size, int64_t pool_pages,

@@ -503,3 +503,26 @@ def test_a_wait_that_runs_out_ends_the_launch_and_is_reported():
         assert F.decode_status() == 0
         assert torch.equal(F.gqa_decode_int4(q, pages, lens, table, page_size=16), want)
     assert F.decode_status() == 0
+
+
+def test_a_wait_that_runs_out_in_a_graph_is_reported():
+    """The counters of a captured call are the graph's own and are cleared on every replay; what went wrong is kept."""
+    q, pages, lens, table = make([60000, 3000, 500], 32, 8, 128, 16, seed=22)
+    want = F.gqa_decode_int4(q, pages, lens, table, page_size=16)
+    graphs = []
+    for config in ({"wait_log2": 1}, None):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = F.gqa_decode_int4(q, pages, lens, table, page_size=16, config=config)
+        graphs.append((graph, out))
+    assert F.decode_status() == 0
+    (short, _), (good, out) = graphs
+    for _ in range(2):
+        short.replay()
+        good.replay()                    # a good launch behind it does not hide it
+        torch.cuda.synchronize()
+        assert F.decode_status() in (601, 602, 603)
+        assert F.decode_status() == 0
+        assert torch.equal(out, want)
+    good.replay()
+    assert F.decode_status() == 0

@@ -248,3 +248,8 @@ def test_decode_flags_of_the_wait_limit():
     for bad in (-1, 32):
         with pytest.raises(ValueError, match="wait_log2"):
             _native.decode_flags({"wait_log2": bad})
+
+
+def test_status_of_the_4_bit_decode_wants_a_place_for_the_code():
+    assert _native.lib().tb200_gqa_decode_int4_status(None, 0, None) == 1
+    assert F.decode_status("cpu") == 0

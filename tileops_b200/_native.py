@@ -149,6 +149,7 @@ SIGNATURES = {
         c_void_p, c_void_p, c_void_p, c_void_p,                         # k_new v_new k_out v_out
         c_int, c_int, c_int, c_int, c_int, c_int, c_int64, c_void_p]),  # dtype total B Hkv D page pool_pages stream
     "tb200_gqa_decode_int4_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "tb200_gqa_decode_int4_status": (c_int, [c_void_p, c_int, c_void_p]),   # code reset stream
     "tb200_gqa_decode_int4": (c_int, [
         c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,               # q kv_pages o lse lens
         c_void_p, c_int64, c_int, c_int, c_int,                        # table stride width q_dtype o_dtype

@@ -242,6 +242,10 @@ __device__ __forceinline__ void mma_16832_u8s8(int (&d)[4], const uint32_t (&a)[
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
 
+// Code of the first wait on this device that ran out since the word was last cleared.  The workspace has one too, but that of a
+// captured launch is a temporary of the graph, which clears it on every replay: this one stays until the host reads it.
+__device__ int g_gave_up;
+
 // As mbar_wait_bounded, with the first poll in line.
 __device__ __forceinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code,
                                             long long limit, unsigned sleep) {
@@ -252,6 +256,7 @@ __device__ __forceinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, vo
     if (clock64() - t0 > limit) {
       *abort_flag = 1;
       atomicCAS(status, 0, code);
+      atomicCAS(&g_gave_up, 0, code);
       return false;
     }
   }
@@ -1019,6 +1024,17 @@ using namespace tb200;
 extern "C" size_t tb200_gqa_decode_int4_workspace_bytes(int batch, int heads, int heads_kv, int dim) {
   if (batch <= 0 || heads <= 0 || heads_kv <= 0 || heads % heads_kv != 0 || (dim != 64 && dim != 128)) return 0;
   return make_layout(batch, heads, heads_kv, dim).total;
+}
+
+extern "C" int tb200_gqa_decode_int4_status(int32_t* code, int reset, void* stream) {
+  if (!code) TB200_FAIL(TB200_ERR_BAD_ARGUMENT, "code must be non-null");
+  void* word = nullptr;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  TB200_CUDA_CHECK(cudaGetSymbolAddress(&word, g_gave_up));
+  TB200_CUDA_CHECK(cudaMemcpyAsync(code, word, sizeof(int32_t), cudaMemcpyDeviceToHost, s));
+  TB200_CUDA_CHECK(cudaStreamSynchronize(s));
+  if (reset && *code) TB200_CUDA_CHECK(cudaMemsetAsync(word, 0, sizeof(int32_t), s));
+  return TB200_OK;
 }
 
 extern "C" int tb200_gqa_decode_int4(const void* q, const void* kv_pages, void* o, float* lse,

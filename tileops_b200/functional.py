@@ -7,6 +7,7 @@ synchronise with the device.
 
 from __future__ import annotations
 
+import ctypes
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -235,15 +236,21 @@ def prefill_status(device: "torch.device | str | int | None" = None, reset: bool
 
 
 def decode_status(device: "torch.device | str | int | None" = None) -> int:
-    """Largest non-zero status word left by a decode launch in any cached workspace of ``device`` (601-603:
-    a bounded wait of the TMA decode kernel ran out), else 0.  Synchronises.  A workspace whose status is set
-    is dropped from the cache (its counters are no longer trustworthy); the next call allocates a fresh one."""
+    """Largest non-zero status word left by a decode launch in any cached workspace of ``device`` (601-603: a bounded wait
+    of the TMA decode kernel or of the 4-bit decode ran out), or by a 4-bit decode in a replayed CUDA graph, else 0.
+    Synchronises with the current stream; launches and replays on other streams have to be waited for first.  A workspace
+    whose status is set is dropped from the cache (its counters are no longer trustworthy) and the next call allocates a
+    fresh one; a graph clears its own counters on every replay."""
     dev, worst = _device_of(device), 0
     for key in [k for k in _WORKSPACES if len(k) > 2 and k[2] == "decode" and k[0] == dev]:
         code = int(_WORKSPACES[key][8:12].view(torch.int32).item())
         if code:
             worst = max(worst, code)
             del _WORKSPACES[key]
+    if dev.type == "cuda" and torch.cuda.is_initialized():
+        code = ctypes.c_int32(0)
+        N.check(N.launch(dev, N.lib().tb200_gqa_decode_int4_status, ctypes.addressof(code), 1), "tb200_gqa_decode_int4_status")
+        worst = max(worst, code.value)
     return worst
 
 
@@ -823,7 +830,8 @@ def _capturing(device: torch.device) -> bool:
 def _decode_int4_workspace(device: torch.device, batch: int, heads: int, heads_kv: int, dim: int) -> torch.Tensor:
     """Scratch of the 4-bit decode.  Eager calls keep one buffer per (device, stream, shape), as the other decode calls do.
     A call under capture gets one of its own from the graph's pool, cleared by a node of the graph: two graphs, or a
-    graph and an eager call, that run at the same time then never share counters."""
+    graph and an eager call, that run at the same time then never share counters.  A wait that runs out in such a launch is
+    recorded outside the buffer as well (:func:`decode_status`)."""
     capturing = _capturing(device)
     key = (device, torch._C._cuda_getCurrentRawStream(device.index), "decode", batch, heads, heads_kv, dim, "int4")
     ws = None if capturing else _WORKSPACES.get(key)
