@@ -11,6 +11,7 @@ from tileops_b200 import _native
 from tileops_b200 import functional as F
 from tileops_b200 import ops
 from tileops_b200.kernels import Kernel
+from tileops_b200.manifest import load_manifest
 from tileops_b200.perf import formulas
 
 I4Decode = ops.GroupedQueryAttentionDecodePagedInt4KVCacheFwdOp
@@ -253,3 +254,75 @@ def test_decode_flags_of_the_wait_limit():
 def test_status_of_the_4_bit_decode_wants_a_place_for_the_code():
     assert _native.lib().tb200_gqa_decode_int4_status(None, 0, None) == 1
     assert F.decode_status("cpu") == 0
+
+
+# ---- manifest ------------------------------------------------------------------------------------------------------------
+FAMILY = ["PagedKVCachePlanFwdOp", "PagedKVCacheReleaseFwdOp", "QKNormRopeFwdOp", "QKNormRopeKVCacheAppendFwdOp",
+          "QKNormRopeInt4KVCacheAppendFwdOp", "Int4KVCacheAppendFwdOp", "Int4KVCacheGatherFwdOp",
+          "GroupedQueryAttentionDecodePagedInt4KVCacheFwdOp", "GroupedQueryAttentionPrefillPagedInt4KVCacheFwdOp"]
+
+
+def make_op(name, kernel=None):
+    args = {"PagedKVCachePlanFwdOp": (2, 2, 16), "PagedKVCacheReleaseFwdOp": (2, 2, 16), "QKNormRopeFwdOp": (8, 2, 64, 32),
+            "QKNormRopeKVCacheAppendFwdOp": (8, 2, 64), "QKNormRopeInt4KVCacheAppendFwdOp": (8, 2, 64, 16),
+            "Int4KVCacheAppendFwdOp": (2, 64, 16), "Int4KVCacheGatherFwdOp": (2, 64, 16, torch.float16),
+            "GroupedQueryAttentionDecodePagedInt4KVCacheFwdOp": (2, 8, 2, 64, 64, 16),
+            "GroupedQueryAttentionPrefillPagedInt4KVCacheFwdOp": (2, 8, 2, 2, 16, 64)}[name]
+    cls = getattr(ops, name)
+    slot = load_manifest()[name]["source"]["kernel_map"]
+    return cls(*args, kernel_map={key: kernel for key in slot} if kernel else None)
+
+
+@pytest.mark.parametrize("name", FAMILY)
+def test_every_operator_of_the_step_has_a_manifest_entry(name):
+    entry = load_manifest()[name]
+    assert name in ops.__all__ and entry["roofline"]["func"].split(".")[-1] in formulas.__all__
+    assert entry["source"]["kernel_map"] == {k: c.__name__ for k, c in make_op(name).kernel_map.items()}
+    for label in entry["workloads"]:
+        work = {k: v for k, v in label.items() if k not in ("label", "dtypes")}
+        flops, nbytes = getattr(formulas, entry["roofline"]["func"].split(".")[-1])(
+            **(dict(batch=128, heads=64, heads_kv=8, seqlen_kv=524288, dim=128) if "q_shape" in work else {}), **work)
+        assert flops >= 0 and nbytes > 0
+    params = make_op(name)._manifest_params()
+    assert list(params) == list(entry["signature"]["params"])
+
+
+def test_manifest_params_reach_a_builder():
+    assert make_op("GroupedQueryAttentionPrefillPagedInt4KVCacheFwdOp")._manifest_params() == {
+        "max_pages_per_req": 2, "page_size": 16, "is_causal": True, "sm_scale": 64 ** -0.5, "softcap": 0.0}
+    assert make_op("QKNormRopeInt4KVCacheAppendFwdOp")._manifest_params() == {
+        "page_size": 16, "rotary_dim": 64, "rope_base": 10000.0, "eps": 1e-6, "inv_freq": None}
+    assert make_op("Int4KVCacheGatherFwdOp")._manifest_params() == {"dim": 64, "page_size": 16, "dtype": torch.float16}
+
+
+def test_rooflines_of_the_step():
+    q, k = torch.zeros(5, 8, 64, dtype=torch.bfloat16), torch.zeros(5, 2, 64, dtype=torch.bfloat16)
+    slots, pool = torch.zeros(5, dtype=torch.int32), torch.zeros(4, 2, 16 * 72, dtype=torch.uint8)
+    lens, table = torch.zeros(2, dtype=torch.int32), torch.zeros(2, 2, dtype=torch.int32)
+    op = make_op("QKNormRopeFwdOp", _Recorder)
+    with pytest.raises(RuntimeError, match="after a forward"):
+        op.eval_roofline()
+    op(q, k, None, None, slots)
+    assert op.eval_roofline() == (50 * (4 * 64 + 3 * 32), 2 * 50 * 64 * 2 + 5 * 4 + 2 * 64 * 2)
+    op = make_op("QKNormRopeKVCacheAppendFwdOp", _Recorder)
+    op(q, k, k, None, None, slots, slots, k, k)
+    want = (50 * 7 * 64, 2 * 50 * 64 * 2 + 5 * 4 + 256 + 2 * 10 * 64 * 2 + 5 * 4)
+    assert op.eval_roofline() == want
+    op = make_op("QKNormRopeInt4KVCacheAppendFwdOp", _Recorder)
+    op(q, k, k, None, None, slots, slots, pool)
+    assert op.eval_roofline() == (want[0], want[1] - 2 * 10 * 64 * 2 + 10 * 72)
+    op = make_op("Int4KVCacheAppendFwdOp", _Recorder)
+    op(k, k, slots, pool)
+    assert op.eval_roofline() == (8 * 10 * 64, 10 * (256 + 72) + 20)
+    op = make_op("Int4KVCacheGatherFwdOp", _Recorder)
+    op(pool, table, torch.zeros(3, dtype=torch.int32), 20)
+    assert op.eval_roofline() == (4 * 40 * 64, 40 * (256 + 72) + 8)
+    op = make_op("PagedKVCachePlanFwdOp", _Recorder)
+    op(lens, lens, table, None, None, 20)
+    assert op.eval_roofline() == (0, 4 * (10 + 1 + 4 + 40))
+    assert make_op("PagedKVCacheReleaseFwdOp").eval_roofline() == (0, 2 * (9 + 16))
+    work = dict(total_q=24, batch=2, q_lens=[20, 4], cache_lens=[7, 30], heads=8, heads_kv=2, dim=64, page_size=16,
+                max_pages_per_req=3, max_seqlen_q=20, is_causal=True, dtype=torch.bfloat16)
+    flops, nbytes = formulas.gqa_prefill_paged_with_kv_cache_fwd_roofline(**work)
+    # of the 16-bit form's K and V, those read from the cache (37 tokens) and those appended (24) have 72 bytes a head
+    assert formulas.gqa_prefill_paged_int4_roofline(**work) == (flops, nbytes - (37 + 24) * 2 * (256 - 72))

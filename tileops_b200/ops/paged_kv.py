@@ -84,6 +84,7 @@ class PagedKVCachePlanFwdOp(Op):
     def forward(self, seq_lens, new_lens, block_table, free_pages, free_count, total_tokens: int,
                 inplace: bool = False) -> PagedKVPlan:
         self._check(seq_lens, block_table)
+        self.total_tokens = int(total_tokens)
         return self._kernel("paged_kv_plan_kernel", (seq_lens, new_lens, block_table, free_pages, free_count))(
             seq_lens, new_lens, block_table, free_pages, free_count, total_tokens, inplace=inplace)
 
@@ -127,7 +128,7 @@ class QKNormRopeFwdOp(Op):
         if not eps >= 0:
             raise ValueError("eps must be non-negative")
         self.heads, self.heads_kv, self.dim = heads, heads_kv, dim
-        self.rotary_dim, self.rope_base, self.eps = rotary_dim, rope_base, eps
+        self.rotary_dim, self.rope_base, self.eps, self.inv_freq = rotary_dim, rope_base, eps, inv_freq
         half = rotary_dim // 2
         if inv_freq is None:
             turns = [rope_base ** (-j / half) / (2 * math.pi) for j in range(half)]
@@ -164,6 +165,7 @@ class QKNormRopeFwdOp(Op):
             raise ValueError(f"q must have shape [T, {self.heads}, {self.dim}], got {tuple(q.shape)}")
         if k.shape[1:] != (self.heads_kv, self.dim):
             raise ValueError(f"k must have shape [T, {self.heads_kv}, {self.dim}], got {tuple(k.shape)}")
+        self.total_tokens, self.dtype = q.shape[0], q.dtype       # for eval_roofline
 
     def forward(self, q, k, q_weight, k_weight, positions) -> tuple:
         self._check(q, k)
@@ -238,6 +240,7 @@ class Int4KVCacheAppendFwdOp(Op):
     def forward(self, k, v, slot_mapping, kv_pages) -> None:
         if k.shape[1:] != (self.heads_kv, self.dim):
             raise ValueError(f"k must have shape [T, {self.heads_kv}, {self.dim}], got {tuple(k.shape)}")
+        self.total_tokens, self.dtype = k.shape[0], k.dtype
         slot = "int4_kv_cache_append_kernel"
         self.get_or_build_kernel(slot, (k, v, slot_mapping, kv_pages),
                                  build=lambda: self.kernel_map[slot](self.dim, self.page_size))(
@@ -266,6 +269,7 @@ class Int4KVCacheGatherFwdOp(Op):
         if kv_pages.ndim != 3 or kv_pages.shape[1] != self.heads_kv:
             raise ValueError(f"kv_pages must be [pages, {self.heads_kv}, {int4_page_bytes(self.page_size, self.dim)}], "
                              f"got {tuple(kv_pages.shape)}")
+        self.total_tokens = int(total_tokens)
         slot = "int4_kv_cache_gather_kernel"
         return self.get_or_build_kernel(slot, (kv_pages, block_table, cu_seqlens_kv),
                                         build=lambda: self.kernel_map[slot](self.dim, self.page_size, self.dtype))(

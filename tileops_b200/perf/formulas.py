@@ -23,6 +23,15 @@ __all__ = [
     "gqa_prefill_paged_with_kv_cache_fwd_roofline",
     "gqa_decode_roofline",
     "gqa_decode_paged_roofline",
+    "gqa_decode_paged_int4_roofline",
+    "gqa_prefill_paged_int4_roofline",
+    "paged_kv_plan_roofline",
+    "paged_kv_release_roofline",
+    "qk_norm_rope_roofline",
+    "qk_norm_rope_append_roofline",
+    "qk_norm_rope_int4_append_roofline",
+    "int4_kv_cache_append_roofline",
+    "int4_kv_cache_gather_roofline",
 ]
 
 
@@ -186,3 +195,86 @@ def gqa_decode_paged_int4_roofline(op: Any = None, **kwargs: Any) -> tuple:
     meta = batch * 4 + batch * max(1, -(-seqlen_kv // page)) * 4
     return (int(4 * batch * heads * seqlen_kv * dim),
             int(2 * batch * heads * dim * _itemsize(_dtype_of(d)) + seqlen_kv * heads_kv * (dim + 8) + meta))
+
+
+def gqa_prefill_paged_int4_roofline(op: Any = None, **kwargs: Any) -> tuple:
+    """Packed prefill over a 4-bit cache with append: the flops of the 16-bit one; of its bytes, the cached K/V read and the
+    chunk's K/V written are ``dim + 8`` per token and KV head."""
+    d = dict(_fields(op, kwargs))
+    flops, nbytes = gqa_prefill_paged_with_kv_cache_fwd_roofline(d)
+    heads_kv, dim = int(d["heads_kv"]), int(d["dim"])
+    e = _itemsize(_dtype_of(d))
+    batch, max_q = int(d["batch"]), int(d.get("max_seqlen_q", int(d["max_pages_per_req"]) * int(d["page_size"])))
+    q_lens = d.get("q_lens")
+    total_q = int(d["total_q"]) if "total_q" in d else (int(sum(q_lens)) if q_lens is not None else batch * max_q)
+    if q_lens is None:
+        q_lens = _spread(total_q, batch, max_q)
+    cache_lens = d.get("cache_lens")
+    if cache_lens is None:
+        cap = int(d["max_pages_per_req"]) * int(d["page_size"])
+        cache_lens = [max(cap - int(n), 0) for n in q_lens]
+    tokens = sum(int(n) for n in cache_lens) + total_q          # in 4 bits instead of 16
+    return flops, int(nbytes - tokens * heads_kv * (2 * dim * e - (dim + 8)))
+
+
+def _total_tokens(d: dict) -> int:
+    if d.get("total_tokens") is None:
+        raise RuntimeError("the row count is known after a forward() call: total_tokens is not set")
+    return int(d["total_tokens"])
+
+
+def paged_kv_plan_roofline(op: Any = None, **kwargs: Any) -> tuple:
+    """Plan of a step: two lengths in, two words, a row offset and a grant out per request, slot and position per row, and
+    the pages that ``total_tokens`` new tokens fill, taken off the stack and entered in the table."""
+    d = _fields(op, kwargs)
+    batch, page, tokens = int(d["batch"]), int(d["page_size"]), _total_tokens(d)
+    return 0, int(4 * (5 * batch + 1 + 2 * (-(-tokens // page)) + 2 * tokens))
+
+
+def paged_kv_release_roofline(op: Any = None, **kwargs: Any) -> tuple:
+    """Release with every request finished and its table full: a flag and a length in and a length out per request, and
+    every page from the table to the stack."""
+    d = _fields(op, kwargs)
+    return 0, int(d["batch"]) * (9 + 8 * int(d["max_pages_per_req"]))
+
+
+def qk_norm_rope_roofline(op: Any = None, **kwargs: Any) -> tuple:
+    """Norm and rotation: q and k in and out, a position per token, the weights."""
+    d = _fields(op, kwargs)
+    heads, heads_kv, dim = (int(d[k]) for k in ("heads", "heads_kv", "dim"))
+    tokens, e = _total_tokens(d), _itemsize(_dtype_of(d))
+    rows = tokens * (heads + heads_kv)
+    return rows * (4 * dim + 3 * int(d["rotary_dim"])), int(2 * rows * dim * e + 4 * tokens + 2 * dim * e)
+
+
+def qk_norm_rope_append_roofline(op: Any = None, **kwargs: Any) -> tuple:
+    """The same with the append: v in and out besides, and a slot per token (k goes to the cache alone)."""
+    d = _fields(op, kwargs)
+    flops, nbytes = qk_norm_rope_roofline(d)
+    tokens, heads_kv, dim = _total_tokens(d), int(d["heads_kv"]), int(d["dim"])
+    return flops, nbytes + tokens * (2 * heads_kv * dim * _itemsize(_dtype_of(d)) + 4)
+
+
+def qk_norm_rope_int4_append_roofline(op: Any = None, **kwargs: Any) -> tuple:
+    """The same with k and v stored in 4 bits: ``dim + 8`` bytes per token and KV head."""
+    d = _fields(op, kwargs)
+    flops, nbytes = qk_norm_rope_append_roofline(d)
+    tokens, heads_kv, dim = _total_tokens(d), int(d["heads_kv"]), int(d["dim"])
+    return flops, nbytes - tokens * heads_kv * (2 * dim * _itemsize(_dtype_of(d)) - (dim + 8))
+
+
+def int4_kv_cache_append_roofline(op: Any = None, **kwargs: Any) -> tuple:
+    """Quantising append: K and V in 16 bits in, ``dim + 8`` bytes per token and KV head out, a slot per token; four
+    operations a value."""
+    d = _fields(op, kwargs)
+    tokens, heads_kv, dim = _total_tokens(d), int(d["heads_kv"]), int(d["dim"])
+    return 8 * tokens * heads_kv * dim, int(tokens * (heads_kv * (2 * dim * _itemsize(_dtype_of(d)) + dim + 8) + 4))
+
+
+def int4_kv_cache_gather_roofline(op: Any = None, **kwargs: Any) -> tuple:
+    """Read-back: ``dim + 8`` bytes per token and KV head in, K and V in 16 bits out, a table entry per page; a multiply-add a
+    value."""
+    d = _fields(op, kwargs)
+    tokens, heads_kv, dim, page = _total_tokens(d), int(d["heads_kv"]), int(d["dim"]), int(d["page_size"])
+    return (4 * tokens * heads_kv * dim,
+            int(tokens * heads_kv * (2 * dim * _itemsize(_dtype_of(d)) + dim + 8) + 4 * (-(-tokens // page))))
