@@ -326,3 +326,12 @@ def test_rooflines_of_the_step():
     flops, nbytes = formulas.gqa_prefill_paged_with_kv_cache_fwd_roofline(**work)
     # of the 16-bit form's K and V, those read from the cache (37 tokens) and those appended (24) have 72 bytes a head
     assert formulas.gqa_prefill_paged_int4_roofline(**work) == (flops, nbytes - (37 + 24) * 2 * (256 - 72))
+
+
+def test_tables_that_pages_are_entered_in_have_rows_of_their_own():
+    F._check_rows_apart(torch.zeros(3, 4, dtype=torch.int32))
+    F._check_rows_apart(torch.zeros(3, 9, dtype=torch.int32)[:, 2:6])
+    F._check_rows_apart(torch.zeros(1, 4, dtype=torch.int32).expand(1, 4))
+    for bad in (torch.zeros(1, 4, dtype=torch.int32).expand(3, 4), torch.zeros(12, dtype=torch.int32).as_strided((3, 4), (2, 1))):
+        with pytest.raises(ValueError, match="must not overlap"):
+            F._check_rows_apart(bad)

@@ -511,3 +511,12 @@ def test_rows_whose_step_is_a_subnormal_keep_the_stated_bound():
     tol = step / 2 + 15 * rounding(step) + rounding(x.amax(-1, keepdim=True)) + rounding(x.abs() + step)
     assert_within(k, x, tol, "k")
     assert_within(v, -x, tol, "v")
+
+
+def test_plan_refuses_to_enter_pages_in_a_row_that_requests_share():
+    shared = i32([[1, 2, 3]]).expand(2, 3)
+    with pytest.raises(ValueError, match="must not overlap"):
+        ops.PagedKVCachePlanFwdOp(2, 3, 16)(i32([0, 0]), i32([1, 1]), shared, i32([4, 5]), i32([2]), 2)
+    # a table that is only read may be shared
+    plan = ops.PagedKVCachePlanFwdOp(2, 3, 16)(i32([17, 3]), i32([1, 1]), shared, None, None, 2)
+    assert plan.slot_mapping.tolist() == [2 * 16 + 1, 16 + 3]

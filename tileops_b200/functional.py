@@ -545,6 +545,12 @@ def _check_table(block_table: torch.Tensor, batch: int, device: torch.device) ->
         raise ValueError("the rows of block_table must be contiguous")
 
 
+def _check_rows_apart(block_table: torch.Tensor) -> None:
+    """New pages are entered in the table: its rows must be places of their own (an expanded row is none)."""
+    if block_table.shape[0] > 1 and block_table.stride(0) < block_table.shape[1]:
+        raise ValueError("the rows of block_table must not overlap where pages are entered in it")
+
+
 def paged_kv_plan(seq_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor,
                   free_pages: Optional[torch.Tensor], free_count: Optional[torch.Tensor], total_tokens: int, *,
                   page_size: int, inplace: bool = False) -> PagedKVPlan:
@@ -567,6 +573,7 @@ def paged_kv_plan(seq_lens: torch.Tensor, new_lens: torch.Tensor, block_table: t
     if free_pages is not None:
         _check_vector("free_pages", free_pages, free_pages.numel(), device)
         _check_vector("free_count", free_count, 1, device)
+        _check_rows_apart(block_table)
     if total < 0:
         raise ValueError("total_tokens must not be negative")
     buf = seq_lens.new_empty(2 * total + 3 * batch + 2)     # one allocation; the slot map, written most, starts it
