@@ -573,7 +573,8 @@ def paged_kv_plan(seq_lens: torch.Tensor, new_lens: torch.Tensor, block_table: t
     if free_pages is not None:
         _check_vector("free_pages", free_pages, free_pages.numel(), device)
         _check_vector("free_count", free_count, 1, device)
-        _check_rows_apart(block_table)
+        if not block_table.is_contiguous():
+            _check_rows_apart(block_table)
     if total < 0:
         raise ValueError("total_tokens must not be negative")
     buf = seq_lens.new_empty(2 * total + 3 * batch + 2)     # one allocation; the slot map, written most, starts it

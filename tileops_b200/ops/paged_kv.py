@@ -161,11 +161,12 @@ class QKNormRopeFwdOp(Op):
         return turns
 
     def _check(self, q, k) -> None:
-        if q.shape[1:] != (self.heads, self.dim):
+        shape = q.shape
+        if shape[1:] != (self.heads, self.dim):
             raise ValueError(f"q must have shape [T, {self.heads}, {self.dim}], got {tuple(q.shape)}")
         if k.shape[1:] != (self.heads_kv, self.dim):
             raise ValueError(f"k must have shape [T, {self.heads_kv}, {self.dim}], got {tuple(k.shape)}")
-        self.total_tokens, self.dtype = q.shape[0], q.dtype       # for eval_roofline
+        self.total_tokens = shape[0]       # for eval_roofline
 
     def forward(self, q, k, q_weight, k_weight, positions) -> tuple:
         self._check(q, k)
@@ -240,7 +241,7 @@ class Int4KVCacheAppendFwdOp(Op):
     def forward(self, k, v, slot_mapping, kv_pages) -> None:
         if k.shape[1:] != (self.heads_kv, self.dim):
             raise ValueError(f"k must have shape [T, {self.heads_kv}, {self.dim}], got {tuple(k.shape)}")
-        self.total_tokens, self.dtype = k.shape[0], k.dtype
+        self.total_tokens = k.shape[0]
         slot = "int4_kv_cache_append_kernel"
         self.get_or_build_kernel(slot, (k, v, slot_mapping, kv_pages),
                                  build=lambda: self.kernel_map[slot](self.dim, self.page_size))(
