@@ -335,3 +335,11 @@ def test_tables_that_pages_are_entered_in_have_rows_of_their_own():
     for bad in (torch.zeros(1, 4, dtype=torch.int32).expand(3, 4), torch.zeros(12, dtype=torch.int32).as_strided((3, 4), (2, 1))):
         with pytest.raises(ValueError, match="must not overlap"):
             F._check_rows_apart(bad)
+
+
+def test_the_first_call_of_a_rotation_is_refused_under_capture(monkeypatch):
+    monkeypatch.setattr(F, "_capturing", lambda device: True)
+    op = ops.QKNormRopeFwdOp(8, 2, 64)
+    with pytest.raises(RuntimeError, match="call it once before the capture"):
+        op._turns(torch.device("cuda", 0))
+    assert ops.QKNormRopeFwdOp(8, 2, 64, 0)._turns(torch.device("cuda", 0)) is None

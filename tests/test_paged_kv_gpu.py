@@ -520,3 +520,20 @@ def test_plan_refuses_to_enter_pages_in_a_row_that_requests_share():
     # a table that is only read may be shared
     plan = ops.PagedKVCachePlanFwdOp(2, 3, 16)(i32([17, 3]), i32([1, 1]), shared, None, None, 2)
     assert plan.slot_mapping.tolist() == [2 * 16 + 1, 16 + 3]
+
+
+def test_a_rotation_is_captured_after_its_first_call():
+    T, H, Hkv, D = 3, 4, 2, 64
+    q, k, _, qw, kw = qkv(T, H, Hkv, D, torch.bfloat16, 2)
+    pos = i32([5, 6, 7])
+    op = ops.QKNormRopeFwdOp(H, Hkv, D)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="call it once before the capture"):
+        with torch.cuda.graph(graph):
+            op(q, k, qw, kw, pos)
+    want = op(q, k, qw, kw, pos)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = op(q, k, qw, kw, pos)
+    graph.replay()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

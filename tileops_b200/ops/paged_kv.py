@@ -9,7 +9,8 @@ tables and rotated keys.  A decode step is
     q = QKNormRopeInt4KVCacheAppendFwdOp(...)(q, k, v, q_weight, k_weight, plan.positions, plan.slot_mapping, kv_pages)
     o = GroupedQueryAttentionDecodePagedInt4KVCacheFwdOp(...)(q, kv_pages, plan.seq_lens, block_table)
 
-No call synchronises the host with the device, and each can be captured into a CUDA graph.
+No call synchronises the host with the device, and each can be captured into a CUDA graph; an operator that rotates has to
+have been called on the device once before, since its first call copies the frequencies there.
 """
 
 from __future__ import annotations
@@ -19,6 +20,7 @@ from typing import Dict, Optional
 
 import torch
 
+from .. import functional
 from ..functional import PagedKVPlan, int4_page_bytes
 from ..kernels import (
     Int4KVCacheAppendSm100Kernel,
@@ -113,7 +115,8 @@ class QKNormRopeFwdOp(Op):
     Computed in fp32 with angles in fp64 and rounded once, so there is no cos / sin table and no largest position.
     ``inv_freq`` (``[rotary_dim / 2]``) replaces ``rope_base ** (-2 j / rotary_dim)``, for scaled rotations.  q, k and v may
     be parts of one projection's output (rows on 16-byte boundaries are read where they are).  ``dim`` is a multiple of 8
-    up to 256, ``rotary_dim`` a multiple of 16 up to ``dim``, or 0.
+    up to 256, ``rotary_dim`` a multiple of 16 up to ``dim``, or 0.  The first call on a device copies the frequencies there and
+    cannot be captured.
     """
 
     def __init__(self, heads: int, heads_kv: int, dim: int, rotary_dim: Optional[int] = None, rope_base: float = 10000.0,
@@ -151,11 +154,14 @@ class QKNormRopeFwdOp(Op):
             self.dim, self.eps, page_size=self._page_size))
 
     def _turns(self, device: torch.device) -> Optional[torch.Tensor]:
-        """Frequencies in turns on ``device``: copied there by the first call (which must not be under capture)."""
+        """Frequencies in turns on ``device``, copied there by the first call."""
         if self.rotary_dim == 0:
             return None
         turns = self._inv_turns_on.get(device)
         if turns is None:
+            if device.type == "cuda" and functional._capturing(device):
+                raise RuntimeError(f"the first call of a {type(self).__name__} on a device copies its frequencies there, which a "
+                                   "CUDA graph cannot hold: call it once before the capture")
             turns = self._inv_turns.to(device)
             self._inv_turns_on[device] = turns
         return turns
