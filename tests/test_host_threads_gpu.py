@@ -87,3 +87,30 @@ def test_cp_async_decode_of_a_large_and_of_a_small_batch(fp8):
     alternate(decode_call(300, fp8, {"tma": False}), decode_call(3, fp8, {"tma": False}))
     decode_call(3, fp8, {"tma": False})()
     assert F.decode_last_kernel() == "cp_async"
+
+
+def test_two_prefills_over_an_fp8_cache_whose_launches_interleave(monkeypatch):
+    """Another call of the same shape on the same stream between this call's read-back and its attention must leave this call's
+    keys and values alone."""
+    H, Hkv, D, page, T = 8, 2, 128, 64, 9
+
+    def problem(seed):
+        g = torch.Generator().manual_seed(seed)
+        q, k, v = (torch.randn(T, h, D, generator=g).bfloat16().to(DEV) for h in (H, Hkv, Hkv))
+        pages = [torch.randn(4 * page, Hkv, D, generator=g).to(torch.float8_e4m3fn).to(DEV) for _ in range(2)]
+        one = torch.ones(1, device=DEV)
+        cu, old, table = (torch.tensor(x, dtype=torch.int32, device=DEV) for x in ([0, 4, 9], [20, 9], [[1, 3], [0, 2]]))
+        return lambda: F.gqa_prefill_paged_fp8_cache(q, k, v, *(p.clone() for p in pages), one, one, cu, old, table, 5, page_size=page)
+
+    call, other = problem(0), problem(1)
+    want, attend, inside = call(), F.gqa_prefill_paged, []
+
+    def interleaved(*args, **kwargs):
+        if not inside:
+            inside.append(True)
+            other()
+        return attend(*args, **kwargs)
+
+    monkeypatch.setattr(F, "gqa_prefill_paged", interleaved)
+    got = call()
+    assert inside and torch.equal(got, want)

@@ -458,15 +458,10 @@ def gqa_prefill_paged_fp8_cache(q: torch.Tensor, k_new: torch.Tensor, v_new: tor
     cu_kv = torch.zeros(B + 1, dtype=torch.int32, device=q.device)
     cu_kv[1:] = torch.cumsum(kv_lens, 0)
     # The packed K/V is sized by what the block table can describe (its width x the page size per request)
-    # plus the chunk: an upper bound known on the host, so that no length is read back from the device.
-    # The buffers are kept per shape (a chunked prefill calls this with the same shapes over and over).
+    # plus the chunk: an upper bound known on the host, so that no length is read back from the device.  It is
+    # the call's own: one kept for the shape would be shared by two host threads whose launches interleave.
     total_kv = B * block_table.shape[1] * int(page_size) + total_q
-    key = (q.device, torch.cuda.current_stream(q.device).cuda_stream, "fp8_cache_packed", total_kv, Hkv, D, q.dtype)
-    bufs = _WORKSPACES.get(key)
-    if bufs is None:
-        bufs = (torch.empty((total_kv, Hkv, D), dtype=q.dtype, device=q.device),
-                torch.empty((total_kv, Hkv, D), dtype=q.dtype, device=q.device))
-        _WORKSPACES[key] = bufs
+    bufs = tuple(torch.empty((total_kv, Hkv, D), dtype=q.dtype, device=q.device) for _ in range(2))
     k_all, v_all = bufs
     lib, stream = N.lib(), N.current_stream(q.device)
     with torch.cuda.device(q.device):
