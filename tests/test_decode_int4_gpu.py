@@ -526,3 +526,114 @@ def test_a_wait_that_runs_out_in_a_graph_is_reported():
         assert torch.equal(out, want)
     good.replay()
     assert F.decode_status() == 0
+
+
+def test_a_request_alone_agrees_with_itself_in_a_batch():
+    """The partition depends on the whole batch, so the sums' order may differ: each side is within its tolerance of 64 bits,
+    and the two within twice that of one another."""
+    lens, H, Hkv, D, page = [1500, 4000, 0, 700, 2222] * 6, 32, 8, 128, 16
+    q, pages, t_lens, table = make(lens, H, Hkv, D, page, seed=4)
+    whole = F.gqa_decode_int4(q, pages, t_lens, table, page_size=page, out_dtype=torch.float32)
+    for b in (0, 1, 2, 8):
+        one = F.gqa_decode_int4(q[b:b + 1], pages, t_lens[b:b + 1], table[b:b + 1], page_size=page, out_dtype=torch.float32)
+        to, _ = tolerances(q[b:b + 1].cpu(), pages.cpu(), lens[b:b + 1], table[b:b + 1].cpu(), page, D ** -0.5, 0.0)
+        assert ((one - whole[b:b + 1]).abs().double().cpu() <= 2 * to).all()
+
+
+@pytest.mark.parametrize("cache", ["16bit", "int4"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_a_captured_step_of_plan_append_and_attend_replays_a_decode_loop(cache, dtype):
+    """The chain over either cache: one graph of the plan (in place), the norm with the append and the attention, replayed with
+    new rows, equals the eager calls bit for bit, and attention in 64 bits over what the cache then holds."""
+    B, H, Hkv, D, page, W, pool = 4, 8, 2, 128, 64, 5, 24
+    g = torch.Generator().manual_seed(3)
+    start = [130, 0, 63, 64]
+    plan = ops.PagedKVCachePlanFwdOp(B, W, page)
+    if cache == "int4":
+        append = ops.QKNormRopeInt4KVCacheAppendFwdOp(H, Hkv, D, page)
+        attend = ops.GroupedQueryAttentionDecodePagedInt4KVCacheFwdOp(B, H, Hkv, pool * page, D, page)
+        empty = (torch.full((pool, Hkv, F.int4_page_bytes(page, D)), 255, dtype=torch.uint8, device=DEV),)
+    else:
+        append = ops.QKNormRopeKVCacheAppendFwdOp(H, Hkv, D)
+        attend = ops.GroupedQueryAttentionDecodePagedWithKVCacheFwdOp(B, H, Hkv, pool * page, D, page)
+        empty = tuple(torch.full((pool * page, Hkv, D), float("nan"), dtype=dtype, device=DEV) for _ in range(2))
+    w = (1 + 0.2 * torch.randn(2, D, generator=g)).to(dtype).to(DEV)
+
+    def rows(T):
+        return torch.randn(T, H + 2 * Hkv, D, generator=g).to(dtype).to(DEV)
+
+    def step(x, s, new):
+        p = plan(s["seq"], new, s["table"], s["free"], s["count"], x.shape[0], inplace=True)
+        q = append(x[:, :H], x[:, H:H + Hkv], x[:, H + Hkv:], w[0], w[1], p.positions, p.slot_mapping, *s["cache"])
+        return q, p
+
+    def decode(x, s):
+        q, p = step(x, s, ones)
+        return q, attend(q, *s["cache"], p.seq_lens, s["table"])
+
+    ones = i32([1] * B)
+    order, first = torch.randperm(pool, generator=g).to(torch.int32).to(DEV), rows(sum(start))
+    states = []
+    for _ in range(2):
+        s = dict(seq=i32([0] * B), table=i32([[-1] * W] * B), free=order.clone(), count=i32([pool]),
+                 cache=tuple(x.clone() for x in empty))
+        step(first, s, i32(start))
+        states.append(s)
+    eager, captured = states
+    x = rows(B)
+    warm = dict(captured, **{k: captured[k].clone() for k in ("seq", "table", "free", "count")}, cache=tuple(c.clone() for c in captured["cache"]))
+    decode(x, warm)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got_q, got_o = decode(x, captured)
+    for n in range(70):
+        x.copy_(rows(B))
+        graph.replay()
+        q, o = decode(x, eager)
+        assert torch.equal(got_q, q) and torch.equal(got_o, o), n
+    assert all(torch.equal(a, b) for a, b in zip((eager["seq"], eager["table"], eager["count"]), (captured["seq"], captured["table"], captured["count"])))
+    lens = [n + 70 for n in start]
+    assert eager["seq"].tolist() == lens
+    table = eager["table"].cpu().long()
+    if cache == "int4":
+        ref, _ = O.decode_ref(q.cpu(), eager["cache"][0].cpu(), lens, table, page)
+    else:
+        k, v = (c.double().cpu() for c in eager["cache"])
+        ref = torch.zeros(B, H, D, dtype=torch.float64)
+        for b, n in enumerate(lens):
+            t = torch.arange(n)
+            at = table[b][t // page] * page + t % page
+            for h in range(H):
+                p = torch.softmax(k[at, h // (H // Hkv)] @ q[b, h].double().cpu() * D ** -0.5, 0)
+                ref[b, h] = p @ v[at, h // (H // Hkv)]
+    torch.testing.assert_close(o.double().cpu(), ref, atol=2e-2, rtol=1e-2)      # the decode tests' own
+
+
+def test_pools_whose_offsets_pass_32_bits():
+    page, Hkv, D, H = 64, 8, 128, 16
+    g = torch.Generator().manual_seed(8)
+    pool = (1 << 32) // (Hkv * F.int4_page_bytes(page, D)) + 40          # bytes of the 4-bit pool
+    pages = torch.empty(pool, Hkv, F.int4_page_bytes(page, D), dtype=torch.uint8, device=DEV)
+    lens = [130, 64]
+    table = i32([[pool - 1, 0, pool - 7], [pool - 2, 3, 5]])
+    T = sum(lens)
+    plan = ops.PagedKVCachePlanFwdOp(2, 3, page)(i32([0, 0]), i32(lens), table, None, None, T)
+    k, v = (torch.randn(T, Hkv, D, generator=g).bfloat16().to(DEV) for _ in range(2))
+    F.int4_cache_append(k, v, plan.slot_mapping, pages, page_size=page)
+    few = torch.zeros(8, *pages.shape[1:], dtype=torch.uint8, device=DEV)     # the same in a small pool
+    small = i32([[7, 0, 1], [6, 3, 5]])
+    slots = ops.PagedKVCachePlanFwdOp(2, 3, page)(i32([0, 0]), i32(lens), small, None, None, T).slot_mapping
+    F.int4_cache_append(k, v, slots, few, page_size=page)
+    q = torch.randn(2, H, D, generator=g).bfloat16().to(DEV)
+    assert torch.equal(F.gqa_decode_int4(q, pages, i32(lens), table, page_size=page), F.gqa_decode_int4(q, few, i32(lens), small, page_size=page))
+    both = [F.int4_cache_gather(p, t, i32([0, 130, 194]), T, dim=D, page_size=page, dtype=torch.bfloat16) for p, t in ((pages, table), (few, small))]
+    assert all(torch.equal(a, b) for a, b in zip(*both))
+    del pages
+    rows = (1 << 31) // (Hkv * D) + 4 * page                              # elements of a 16-bit pool
+    kp, vp = (torch.empty(rows, Hkv, D, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    slots = torch.randperm(page, generator=g).to(torch.int32).to(DEV) + (rows - page)
+    x = torch.randn(page, H + 2 * Hkv, D, generator=g).bfloat16().to(DEV)
+    op = ops.QKNormRopeKVCacheAppendFwdOp(H, Hkv, D)
+    pos = torch.arange(page, dtype=torch.int32, device=DEV)
+    _, k1 = op(x[:, :H], x[:, H:H + Hkv], x[:, H + Hkv:], None, None, pos, slots, kp, vp, return_k=True)
+    assert torch.equal(kp[slots.long()], k1) and torch.equal(vp[slots.long()], x[:, H + Hkv:])
