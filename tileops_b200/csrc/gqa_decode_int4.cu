@@ -29,8 +29,8 @@
 //   * Rows of a record are dealt to the MMA rows in the order 0 7 1 6 2 5 3 4: the pairs a lane needs of V (consecutive k
 //     of the second product) and the rows it reads of K then fall into different banks.
 //   * At most four q heads per KV head leave half of N idle: the second digit of q takes it, the lanes of the two halves
-//     exchange what the other needs and have one token's scores of a record each (64 sequences of 512 to 8192 tokens 67.2 ->
-//     63.5 us).
+//     exchange what the other needs and have one token's scores of a record each (64 sequences of 512 to 8192 tokens, 297 MB,
+//     67.2 -> 63.5 us).
 //   * Three blocks of four math warps per SM (head dim 64: four; two head tiles: two), each with a producer warp that streams records by untiled bulk copies (as many
 //     tokens as a page and a tile have in common, 16 at least) into a ring of shared-memory stages, across segment boundaries.
 //     (One block of twelve math warps, which share every stage and every segment, repeats a segment's beginning and end in
@@ -39,8 +39,8 @@
 //     counts as two or three tiles (without that 78 us instead of 69 on 64 sequences of 512 to 8192 tokens, whose short lanes
 //     made the blocks that got them late).  Partial results of a (sequence, KV head) that ranges share go to global memory
 //     in accumulator order; the last block to finish merges them, at the end of its range.
-// Measured, 32 q and 8 KV heads x 128, bf16, captured: 8 x 131072 tokens 185 us = 6.2 TB/s (214 us back to back, where the
-// board's power limit takes the clock to 1.65 GHz); 64 sequences of 512 to 8192 tokens 67 us = 4.9 TB/s: of that 6 us pass
+// Measured, 32 q and 8 KV heads x 128, bf16, captured: 8 x 131072 tokens 186 us = 6.1 TB/s (205 to 217 us back to back, where
+// the board's power limit takes the clock to 1.65 GHz); 64 sequences of 512 to 8192 tokens, 325 MB, 67 us = 4.9 TB/s: of that 6 us pass
 // before the first tile, 5 after the last, and each segment's begin and end cost its block 3; 1 x 1000 tokens 11 us, latency.
 #include <type_traits>
 
@@ -268,7 +268,7 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
   return mbar_wait_slow(bar, parity, abort_flag, status, code, limit, sleep);
 }
 // The same by a whole warp, whose lanes get one answer: where one of them gives up, none goes on to a shuffle or a vote that
-// it no longer takes part in.
+// it no longer takes part in.  (64 ragged requests, 297 MB, 62.0 -> 62.5 us; 8 x 131072 tokens 184.9 -> 187.0 us.)
 __device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code,
                                                long long limit) {
   if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;

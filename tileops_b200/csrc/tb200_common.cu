@@ -23,4 +23,4 @@ int sm_count() {
 }  // namespace tb200
 
 extern "C" const char* tb200_last_error(void) { return tb200::error_buffer(); }
-extern "C" int tb200_version(void) { return 103; }  // 1.03: paged-KV plan, per-head norm + rotation + append, 4-bit paged KV cache
+extern "C" int tb200_version(void) { return 104; }  // 1.04: status of the 4-bit decode outside its workspace, limit of its waits

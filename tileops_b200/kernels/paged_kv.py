@@ -39,10 +39,6 @@ class PagedKVPlanSm100Kernel(Kernel):
         self.page_size = page_size
         self.init_config(config)
 
-    @property
-    def default_config(self) -> dict:
-        return {"threads": 1024}
-
     def forward(self, seq_lens, new_lens, block_table, free_pages, free_count, total_tokens, inplace=False):
         return F.paged_kv_plan(seq_lens, new_lens, block_table, free_pages, free_count, total_tokens,
                                page_size=self.page_size, inplace=inplace)
@@ -98,6 +94,10 @@ class Int4KVCacheAppendSm100Kernel(_Int4CacheBase):
 
 
 class Int4KVCacheGatherSm100Kernel(_Int4CacheBase):
+    @property
+    def default_config(self) -> dict:
+        return {"threads": 288}
+
     def forward(self, kv_pages, block_table, cu_seqlens_kv, total_tokens):
         return F.int4_cache_gather(kv_pages, block_table, cu_seqlens_kv, total_tokens, dim=self.dim,
                                    page_size=self.page_size, dtype=self.dtype)
@@ -105,7 +105,8 @@ class Int4KVCacheGatherSm100Kernel(_Int4CacheBase):
 
 class GQADecodePagedInt4Sm100Kernel(Kernel):
     """Paged decode over a 4-bit cache: ``forward(Q[B,H,D], kv_pages, real_seqlen_kv[B] i32, block_table[B,W] i32)``.
-    Constructor as :class:`GQADecodePagedFp8Sm100Kernel`."""
+    Constructor as :class:`GQADecodePagedFp8Sm100Kernel`.  ``config`` may set ``chunk_tiles`` (a fixed run length) and
+    ``wait_log2`` (the limit of a device-side wait in clock ticks); ``threads`` describes the kernel."""
 
     supported_archs = [100]
     general = True
@@ -131,7 +132,7 @@ class GQADecodePagedInt4Sm100Kernel(Kernel):
 
     @property
     def default_config(self) -> dict:
-        return {"threads": 128}
+        return {"threads": 160}
 
     def forward(self, Q, kv_pages, real_seqlen_kv, block_table, return_lse: bool = False, out_dtype=None):
         return F.gqa_decode_int4(Q, kv_pages, real_seqlen_kv, block_table, page_size=self.page_size,
@@ -165,6 +166,7 @@ class GQAPrefillPagedInt4CacheSm100Kernel(Kernel):
 
     @property
     def default_config(self) -> dict:
+        """Of the prefill kernel, as its siblings' (fixed)."""
         return {"block_M": 128, "block_N": 64, "threads": 192}
 
     def forward(self, q, k_new, v_new, kv_pages, cu_seqlens_q, cache_seqlens, block_table, max_seqlen_q):
