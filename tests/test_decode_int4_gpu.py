@@ -637,3 +637,13 @@ def test_pools_whose_offsets_pass_32_bits():
     pos = torch.arange(page, dtype=torch.int32, device=DEV)
     _, k1 = op(x[:, :H], x[:, H:H + Hkv], x[:, H + Hkv:], None, None, pos, slots, kp, vp, return_k=True)
     assert torch.equal(kp[slots.long()], k1) and torch.equal(vp[slots.long()], x[:, H + Hkv:])
+
+
+def test_prefill_refuses_a_table_of_more_tokens_than_a_request_may_hold():
+    op, q, k, v, pages, _ = chunk_problem(1, 4)
+    wide = torch.empty(1, 1 << 27, dtype=torch.int32, device=DEV)
+    for width in (1 << 27, (1 << 26) + 1):
+        big = ops.GroupedQueryAttentionPrefillPagedInt4KVCacheFwdOp(1, 8, 2, width, 16, 128)
+        big.validate_inputs = False
+        with pytest.raises(ValueError, match="2\\^30 tokens"):
+            big(q, k, v, pages, i32([0, 4]), i32([3]), wide[:, :width], 4)

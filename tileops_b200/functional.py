@@ -902,12 +902,12 @@ def gqa_prefill_paged_int4_cache(q: torch.Tensor, k_new: torch.Tensor, v_new: to
     if total_q == 0:
         return torch.empty_like(q)
     new_lens = cu_seqlens_q[1:] - cu_seqlens_q[:-1]
+    slots = paged_kv_plan(cache_seqlens, new_lens, block_table, None, None, total_q, page_size=page_size).slot_mapping
     # A request that claims more tokens than its table has (or fewer than none) gets rows of its own that read as NaN: none
     # of the others' move out of the buffer.
     capacity = block_table.shape[1] * int(page_size)
     cu_kv = torch.zeros(B + 1, dtype=torch.int32, device=device)
     cu_kv[1:] = torch.cumsum(cache_seqlens.clamp(0, capacity) + new_lens, 0)
-    slots = paged_kv_plan(cache_seqlens, new_lens, block_table, None, None, total_q, page_size=page_size).slot_mapping
     total_kv = B * capacity + total_q
     # The call's own: a buffer kept for the shape would be shared by two host threads whose launches interleave.
     bufs = tuple(torch.empty((total_kv, Hkv, D), dtype=q.dtype, device=device) for _ in range(2))
